@@ -21,7 +21,8 @@ INL_MEM_HOST = 0
 INL_MEM_DEVICE = 1
 
 EPI_BF16, EPI_RESID, EPI_GATED, EPI_F32 = 0, 1, 2, 3
-ACT_SILU, ACT_GELU_ERF, ACT_GELU_TANH = 0, 1, 2
+ACT_SILU, ACT_GELU_ERF, ACT_GELU_TANH, ACT_NONE, ACT_RELU, ACT_TANH = 0, 1, 2, 3, 4, 5
+ROPE_DEFAULT, ROPE_LINEAR, ROPE_DYNAMIC, ROPE_YARN, ROPE_LLAMA3, ROPE_LONGROPE = 0, 1, 2, 3, 4, 5
 
 # Every symbol the two public headers declare.
 EXPORTED = (
@@ -34,7 +35,8 @@ EXPORTED = (
     "inl_cuda_qk_norm_rope", "inl_cuda_token_positions", "inl_cuda_last_token_norm_l2", "inl_cuda_gemm_bf16_ex",
     "inl_cuda_attention_noalloc", "inl_cuda_causal_conv_silu", "inl_cuda_gated_delta_rule",
     "inl_cuda_model_set_dense_normalize", "inl_cuda_config_check", "inl_cuda_model_set_prune_last",
-    "inl_cuda_forward_sparse_compact", "inl_cuda_model_set_f32_gemm",
+    "inl_cuda_forward_sparse_compact", "inl_cuda_model_set_f32_gemm", "inl_cuda_linear",
+    "inl_cuda_rope_frequencies", "inl_cuda_rope", "inl_cuda_qk_norm_rotary",
 )
 
 
@@ -51,6 +53,17 @@ class GemmEx(ctypes.Structure):
         ("sin", ctypes.c_void_p), ("hq", ctypes.c_int), ("hkv", ctypes.c_int), ("d", ctypes.c_int),
         ("max_pos", ctypes.c_int), ("qk_eps", ctypes.c_float), ("force_bn", ctypes.c_int),
         ("status", ctypes.c_void_p),
+    ]
+
+
+class RopeConfig(ctypes.Structure):
+    """Mirror of inl_rope_config (include/inl_cuda_kernels.h)."""
+    _fields_ = [
+        ("type", ctypes.c_int), ("rotary_dim", ctypes.c_int), ("theta", ctypes.c_double), ("factor", ctypes.c_double),
+        ("attention_factor", ctypes.c_double), ("beta_fast", ctypes.c_double), ("beta_slow", ctypes.c_double),
+        ("mscale", ctypes.c_double), ("mscale_all_dim", ctypes.c_double), ("low_freq_factor", ctypes.c_double),
+        ("high_freq_factor", ctypes.c_double), ("short_factor", ctypes.c_void_p), ("long_factor", ctypes.c_void_p),
+        ("original_max_position", ctypes.c_int), ("seq_len", ctypes.c_int), ("no_truncate", ctypes.c_int),
     ]
 
 
@@ -117,6 +130,15 @@ def _declare(lib: ctypes.CDLL) -> None:
         "inl_cuda_gated_delta_rule": (c_int, [c_void_p, c_i64, c_void_p, c_void_p, c_i64, c_void_p, c_i64, c_void_p,
                                               c_void_p, c_void_p, c_float, c_int, c_int, c_int, c_int, c_void_p,
                                               c_int, c_void_p, c_i64, c_void_p]),
+        "inl_cuda_linear": (c_int, [c_void_p, c_i64, c_void_p, c_i64, c_int, c_int, c_int, c_int, c_void_p, c_int,
+                                    c_void_p, c_i64, c_void_p, c_i64, c_int, c_void_p, c_void_p]),
+        "inl_cuda_rope_frequencies": (c_int, [P(RopeConfig), c_void_p, P(c_float)]),
+        "inl_cuda_rope": (c_int, [c_void_p, c_i64, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
+                                  c_float, c_int, c_void_p, c_i64, c_void_p]),
+        "inl_cuda_qk_norm_rotary": (c_int, [c_void_p, c_i64, c_i64, c_void_p, c_i64, c_int, c_int, c_int, c_int,
+                                            c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_int,
+                                            c_int, c_void_p, c_void_p, c_float, c_void_p, c_i64, c_void_p, c_i64,
+                                            c_void_p]),
     }
     for name, (res, args) in sig.items():
         f = getattr(lib, name)

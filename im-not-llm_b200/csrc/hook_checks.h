@@ -1,0 +1,75 @@
+// Argument checks shared by the kernel-level C entry points.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <exception>
+#include <initializer_list>
+#include <string>
+
+#include "../../include/inl_cuda.h"
+
+namespace inl {
+
+int record_error(int code, const std::string& msg);
+
+struct HookPtr {
+  const void* p;
+  int align;  // element size
+  const char* name;
+};
+
+// Every pointer given (NULL ones are the caller's to judge) on an element
+// boundary: no device needed.
+inline int check_aligned(const char* what, std::initializer_list<HookPtr> ptrs) {
+  for (const HookPtr& h : ptrs)
+    if (h.p && (reinterpret_cast<uintptr_t>(h.p) % static_cast<uintptr_t>(h.align)) != 0)
+      return record_error(INL_ERR_INVALID_INPUT, std::string(what) + ": " + h.name + " is not element-aligned");
+  return INL_OK;
+}
+
+// Memory the current device can read: its own, managed, or pinned host
+// memory. A pageable host pointer or another device's memory is refused here,
+// since a kernel that touches it would fault and take the context with it.
+inline int check_reachable(const char* what, std::initializer_list<HookPtr> ptrs) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return record_error(INL_ERR_CONFIG, std::string(what) + ": no CUDA device: " + cudaGetErrorString(e));
+  }
+  for (const HookPtr& h : ptrs) {
+    if (!h.p) continue;
+    cudaPointerAttributes at;
+    e = cudaPointerGetAttributes(&at, h.p);
+    if (e != cudaSuccess) {
+      (void)cudaGetLastError();
+      return record_error(INL_ERR_CONFIG, std::string(what) + ": " + cudaGetErrorString(e));
+    }
+    if (at.type == cudaMemoryTypeUnregistered || (at.type == cudaMemoryTypeDevice && at.device != dev))
+      return record_error(INL_ERR_INVALID_INPUT,
+                          std::string(what) + ": " + h.name + " is not memory of the current device");
+  }
+  return INL_OK;
+}
+
+// Status of a launch: the error is read (and cleared) here.
+inline int launched(const char* what, cudaError_t e) {
+  const cudaError_t last = cudaGetLastError();
+  if (e == cudaSuccess) e = last;
+  if (e == cudaSuccess) return INL_OK;
+  return record_error(INL_ERR_INFERENCE, std::string(what) + " launch failed: " + cudaGetErrorString(e));
+}
+
+// Runs the body of a C entry point; no C++ exception leaves it.
+template <typename F>
+int guarded(F&& body) noexcept {
+  try {
+    return body();
+  } catch (...) {
+    return INL_ERR_INFERENCE;
+  }
+}
+
+}  // namespace inl

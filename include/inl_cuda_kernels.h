@@ -30,6 +30,10 @@ extern "C" {
 #define INL_ACT_SILU_ 0
 #define INL_ACT_GELU_ERF_ 1
 #define INL_ACT_GELU_TANH_ 2
+/* inl_cuda_linear only: */
+#define INL_ACT_NONE_ 3
+#define INL_ACT_RELU_ 4
+#define INL_ACT_TANH_ 5
 
 /* Y[M, N] = X[M, K] . W[N, K]^T on the tcgen05 tensor cores, bf16 operands,
  * f32 accumulation, fused epilogue. Replaces candle's Linear::forward (a cuBLAS
@@ -174,6 +178,109 @@ INL_API int inl_cuda_gated_delta_rule(const float* mixed, int64_t ld_mixed, cons
                                       const float* a_log, const float* norm_w, float eps, int nk, int nv, int dk,
                                       int dv, const int32_t* cu_seqlens_host, int n_texts, float* out, int64_t ldo,
                                       void* stream);
+
+/* Linear layer: out[M, N] = act(x[M, K] . w[N, K]^T + bias[N]) + resid[M, N],
+ * sums, bias, activation and residual in f32 and one rounding at the end.
+ * `dtype` (INL_DTYPE_*) is that of x and w; `out_dtype` that of out and resid;
+ * bias is f32; bias and resid may be NULL. act is any INL_ACT_*_. Any
+ * M, N, K from 0 to 2^30 (K = 0: the product is zero), any row strides >= the
+ * row length, element-aligned pointers; bf16 rows whose addresses are multiples of
+ * 16 bytes (K, ldx, ldw multiples of 8) take the tcgen05 kernels. out may be
+ * resid itself (same pointer and stride); it overlaps nothing else. Nothing
+ * outside the [M, N] elements of out is written. `status` as for
+ * inl_cuda_gemm_bf16. Memory must be reachable from the current device.
+ * Asynchronous on `stream`, no allocation, may be captured. Results do not
+ * change from run to run; they may differ by rounding between M, since the
+ * kernel is chosen by the sizes. Replaces candle_nn::Linear::forward with a
+ * bias followed by the activation and the residual add. */
+INL_API int inl_cuda_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int M, int N, int K,
+                            const float* bias, int act, const void* resid, int64_t ldr, void* out, int64_t ldo,
+                            int out_dtype, int* status, void* stream);
+
+/* Rotary frequencies. `type` picks the scaling for contexts longer than the
+ * trained ones, with the config.json (rope_scaling / rope_parameters) keys
+ * it reads beside theta = rope_theta and rotary_dim = head_dim *
+ * partial_rotary_factor; f_i = theta^(-2i / rotary_dim), i < rotary_dim / 2:
+ *   DEFAULT   f_i
+ *   LINEAR    f_i / factor
+ *   DYNAMIC   f_i with theta' = theta * (factor * L / original - (factor - 1))
+ *             ^ (rotary_dim / (rotary_dim - 2)), L = max(seq_len, original)
+ *   YARN      f_i / factor for slow pairs, f_i for fast ones, a linear ramp over
+ *             i between the pairs that make beta_slow and beta_fast turns in
+ *             `original` positions (bounds rounded outwards unless no_truncate);
+ *             scale = attention_factor, else g(mscale) / g(mscale_all_dim) when
+ *             both are set, else g(1), with g(m) = 0.1 m ln(factor) + 1 (1 when
+ *             factor <= 1)
+ *   LLAMA3    f_i / factor where a turn takes more than original /
+ *             low_freq_factor positions, f_i below original / high_freq_factor,
+ *             interpolated between
+ *   LONGROPE  f_i / short_factor[i], or long_factor[i] when seq_len > original;
+ *             scale = attention_factor, else sqrt(1 + ln(factor) / ln(original))
+ *             (1 when factor <= 1)
+ * scale is 1 for the others. A field left 0 takes its usual value: factor 1,
+ * beta_fast 32, beta_slow 1, low_freq_factor 1, high_freq_factor 4. The
+ * reference accepts the default type alone
+ * (crates/inl-late/src/qwen3_5.rs:56-168, crates/inl-text/src/gemma2.rs:157-164). */
+#define INL_ROPE_DEFAULT 0
+#define INL_ROPE_LINEAR 1
+#define INL_ROPE_DYNAMIC 2
+#define INL_ROPE_YARN 3
+#define INL_ROPE_LLAMA3 4
+#define INL_ROPE_LONGROPE 5
+typedef struct inl_rope_config {
+  int type;
+  int rotary_dim;  /* rotated features of a head, even, > 0 */
+  double theta;    /* > 0 */
+  double factor;
+  double attention_factor; /* 0: the type's own */
+  double beta_fast, beta_slow, mscale, mscale_all_dim;
+  double low_freq_factor, high_freq_factor;
+  const double* short_factor; /* [rotary_dim / 2], LONGROPE */
+  const double* long_factor;
+  int original_max_position; /* YARN, LLAMA3, DYNAMIC, LONGROPE: > 0 (LONGROPE: > 1) */
+  int seq_len;               /* DYNAMIC, LONGROPE: the longest text */
+  int no_truncate;           /* YARN */
+} inl_rope_config;
+
+/* Host only, no device: inv_freq[rotary_dim / 2] (radians per position) and
+ * *scale, for inl_cuda_rope and inl_cuda_qk_norm_rotary. */
+INL_API int inl_cuda_rope_frequencies(const inl_rope_config* config, double* inv_freq, float* scale);
+
+/* Rotary positions on rows of `heads` heads of d features (head h at column
+ * h * d): the first rotary_dim features of each head are rotated in pairs,
+ *   (a, b) -> scale * (a cos t - b sin t, b cos t + a sin t),
+ *   t = pos[token] * inv_freq[i],
+ * pair i being features (i, i + rotary_dim / 2), or (2i, 2i + 1) when
+ * `interleaved`; the other features are copied. `inverse` rotates by -t (the
+ * transpose: undoes a rotation of scale 1, and carries a gradient back).
+ * pos: device int32 [T], any sign; inv_freq: device f64 [rotary_dim / 2]; the
+ * angle is formed and reduced to a quarter turn in 64 bits, so far positions
+ * lose nothing and there is no table. out may be x itself (same pointer and
+ * stride) and overlaps it in no other way. Element-aligned pointers, strides
+ * >= heads * d. Asynchronous on `stream`, no allocation, may be captured.
+ * Replaces candle_nn::rotary_emb::rope and rope_i. */
+INL_API int inl_cuda_rope(const void* x, int64_t ldx, int dtype, int T, int heads, int d, int rotary_dim,
+                          int interleaved, const int32_t* pos, const double* inv_freq, float scale, int inverse,
+                          void* out, int64_t ldo, void* stream);
+
+/* Norms of queries and keys for each head, then the rotation of
+ * inl_cuda_rope, in one pass: RMSNorm x / sqrt(mean x^2 + eps) * w, or
+ * (layer_norm = 1) LayerNorm (x - mean) / sqrt(var + eps) * w + b, over the d
+ * features of each head; qw / kw / qb / kb f32 [d], each may be NULL (no
+ * weight, no bias; biases with LayerNorm only). The normed value is rotated in
+ * f32 and rounded once (inl_cuda_qk_norm_rope rounds in between). q head h of
+ * token t starts at q + t * ldq + h * q_head_stride (>= d: 2 * d reads the
+ * q | gate rows of gated attention), k head h at k + t * ldk + h * d; outputs
+ * have heads at h * d. hq or hkv may be 0 (its pointers are not read). q_out
+ * may be q itself when the strides are equal and q_head_stride = d, k_out may
+ * be k itself; nothing overlaps in any other way. Replaces q_norm / k_norm +
+ * rotary_emb::rope (crates/inl-text/src/qwen3/mod.rs:236-249) and the partial
+ * form of crates/inl-late/src/qwen3_5.rs. */
+INL_API int inl_cuda_qk_norm_rotary(const void* q, int64_t ldq, int64_t q_head_stride, const void* k, int64_t ldk,
+                                    int dtype, int T, int hq, int hkv, int d, int layer_norm, const float* qw,
+                                    const float* qb, const float* kw, const float* kb, float eps, int rotary_dim,
+                                    int interleaved, const int32_t* pos, const double* inv_freq, float scale,
+                                    void* q_out, int64_t ldqo, void* k_out, int64_t ldko, void* stream);
 
 /* Measurement hooks: with profiling on, every GEMM and attention launch of
  * the model is bracketed by CUDA events on the model's stream. kind: 0 qkv,

@@ -1,0 +1,274 @@
+"""inl_cuda_linear (out = act(x w^T + bias) + resid) against the same formula in
+64 bits, and its refusals.
+
+Tolerances, fixed from the arithmetic. u = 2^-24 (half a step of f32).
+* A sum of K products kept in f32 with each add off by at most a whole step
+  (2u of the running value; tensor cores may truncate) is within
+  2u (K + 2) S of the exact one, S = sum |x w| + |bias| (element by element).
+* The activations' slopes are at most 1.13 (gelu), and they are computed to
+  within 2^-19 |v| of the pre-activation value (two hardware approximations of
+  2^-22 each, products and sums of a few roundings, with room); a polynomial
+  argument or an erf of |v| adds nothing larger.
+* One rounding of the result: u |y| (f32) or 2^-9 |y| rounded up to 2^-8 (bf16:
+  half a step is 2^-8 of the value below it), plus the residual add's u.
+* Norm-wise, independent rounding errors add as sqrt(K): the relative 2-norm
+  error of f32 results of random inputs stays below 4 sqrt(K + 16) u.
+"""
+import ctypes
+
+import pytest
+
+F32, BF16 = 0, 1
+ACTS = {"silu": 0, "gelu_erf": 1, "gelu_tanh": 2, "none": 3, "relu": 4, "tanh": 5}
+INVALID, CONFIG = 4, 1
+U = 2.0 ** -24
+
+
+def _n():
+    from im_not_llm_b200 import _native
+
+    return _native
+
+
+def _dt(torch, code):
+    return torch.bfloat16 if code == BF16 else torch.float32
+
+
+def _act64(torch, z, act):
+    import math
+
+    if act == "silu":
+        return z * torch.special.expit(z)
+    if act == "gelu_erf":
+        return z * torch.special.ndtr(z)
+    if act == "gelu_tanh":
+        return 0.5 * z * (1 + torch.tanh(math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)))
+    if act == "relu":
+        return torch.relu(z)
+    return torch.tanh(z) if act == "tanh" else z
+
+
+def _rows(torch, rows, cols, pad, dt, seed, scale=1.0, offset=0):
+    """rows x cols values inside wider rows whose padding is NaN, `offset` elements into their buffer."""
+    g = torch.Generator().manual_seed(seed)
+    ld = cols + pad
+    buf = torch.full((offset + rows * ld,), float("nan"), dtype=_dt(torch, dt))
+    view = buf[offset:].view(rows, ld)[:, :cols]
+    view.copy_(torch.randn(rows, cols, generator=g) * scale)
+    dev = buf.cuda()
+    return dev[offset:].view(rows, ld)[:, :cols], dev
+
+
+def _call(N, torch, x, w, dt, odt, act, bias, resid, out, stream=None, status=None):
+    M, K = x.shape
+    s = torch.cuda.current_stream().cuda_stream if stream is None else stream
+    return N.lib().inl_cuda_linear(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), dt, M, w.shape[0], K,
+                                   None if bias is None else bias.data_ptr(), ACTS[act],
+                                   None if resid is None else resid.data_ptr(),
+                                   0 if resid is None else resid.stride(0), out.data_ptr(), out.stride(0), odt,
+                                   None if status is None else status.data_ptr(), s)
+
+
+def _want(torch, x, w, bias, act, resid):
+    xd, wd = x.double(), w.double()
+    z = xd @ wd.T
+    S = xd.abs() @ wd.abs().T
+    if bias is not None:
+        z, S = z + bias.double(), S + bias.double().abs()
+    y = _act64(torch, z, act)
+    if resid is not None:
+        y = y + resid.double()
+    return z, S, y
+
+
+def _check(torch, got, x, w, bias, act, resid, odt):
+    z, S, y = _want(torch, x, w, bias, act, resid)
+    K = x.shape[1]
+    tol = 1.13 * 2 * U * (K + 2) * S + (0 if act in ("none", "relu") else 2.0 ** -19) * z.abs() + 4 * U * y.abs()
+    if resid is not None:
+        tol = tol + 2 * U * resid.double().abs()
+    if odt == BF16:
+        tol = tol * (1 + 2.0 ** -8) + 2.0 ** -8 * y.abs()
+    err = (got.double() - y).abs()
+    over = (err - tol - 1e-37).max().item() if err.numel() else 0.0
+    assert not torch.isnan(got).any()
+    assert over <= 0, (over, err.max().item())
+    if odt == F32 and y.numel() >= 1024 and act in ("none", "relu", "tanh") and K > 0:
+        rel = ((got.double() - y).norm() / y.norm()).item()
+        assert rel <= 4 * (K + 16) ** 0.5 * U, rel
+
+
+def _one(M, N, K, dt, odt, act, bias, resid, pad=(0, 0, 0, 0), offset=0, seed=1):
+    import torch
+
+    n = _n()
+    x, _ = _rows(torch, M, K, pad[0], dt, seed, 1.0, offset)
+    w, _ = _rows(torch, N, K, pad[1], dt, seed + 1, max(K, 1) ** -0.5, offset)
+    b = torch.randn(N, generator=torch.Generator().manual_seed(seed + 2)).cuda() if bias else None
+    r = _rows(torch, M, N, pad[2], odt, seed + 3, 1.0, offset)[0] if resid else None
+    # a frame of a value that the call must leave alone: a row before and after, padding columns, `offset`
+    ldo = N + pad[3]
+    frame = torch.full((offset + (M + 2) * ldo + 64,), -77.0, device="cuda", dtype=_dt(torch, odt))
+    out = frame[offset + ldo:offset + ldo + M * ldo].view(M, ldo)[:, :N]
+    before = frame.clone()
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    n.check(_call(n, torch, x, w, dt, odt, act, b, r, out, status=st), "linear")
+    torch.cuda.synchronize()
+    assert st.item() == 0
+    _check(torch, out, x, w, b, act, r, odt)
+    inside = torch.zeros_like(frame, dtype=torch.bool)
+    inside[offset + ldo:offset + ldo + M * ldo].view(M, ldo)[:, :N] = True
+    assert torch.equal(frame[~inside], before[~inside])
+    return out
+
+
+# ---------------------------------------------------------------- CPU
+def test_refusals_need_no_gpu():
+    n = _n()
+    f = n.lib().inl_cuda_linear
+
+    def call(x=16, ldx=8, w=16, ldw=8, dt=BF16, M=2, N=2, K=8, bias=None, act=3, resid=None, ldr=2, out=16, ldo=2,
+             odt=BF16, status=None):
+        return f(x, ldx, w, ldw, dt, M, N, K, bias, act, resid, ldr, out, ldo, odt, status, None)
+
+    for bad in (dict(dt=2), dict(odt=-1), dict(M=-1), dict(N=-1), dict(K=-1), dict(K=(1 << 30) + 1), dict(act=6),
+                dict(act=-1), dict(ldx=7), dict(ldw=7), dict(ldo=1), dict(resid=16, ldr=1), dict(ldx=1 << 41),
+                dict(x=17), dict(w=17), dict(out=17), dict(bias=18), dict(resid=19), dict(status=2),
+                dict(dt=F32, x=18), dict(odt=F32, out=18), dict(resid=16, ldr=4, ldo=2)):
+        assert call(**bad) == INVALID, bad
+        assert n.last_error().startswith("linear: ")
+    for null in (dict(x=None), dict(w=None), dict(out=None)):
+        assert call(**null) == CONFIG, null
+        assert "NULL" in n.last_error()
+    # nothing to write: no pointer is read
+    assert call(M=0, x=None, out=None) == 0
+    assert call(N=0, w=None, out=None) == 0
+
+
+# ---------------------------------------------------------------- GPU
+SHAPES = [(1, 1, 1), (1, 4096, 1024), (2, 7, 3), (5, 3, 0), (3, 33, 17), (8, 256, 128), (16, 1000, 520),
+          (17, 1024, 2048), (33, 130, 72), (64, 64, 64), (65, 96, 4096), (129, 513, 264), (300, 768, 768),
+          (257, 72, 1037), (1000, 1021, 100)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_shapes(gpu, M, N, K, dt):
+    _one(M, N, K, dt, dt, "none", True, False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,odt", [(BF16, BF16), (BF16, F32), (F32, F32), (F32, BF16)])
+@pytest.mark.parametrize("act", list(ACTS))
+@pytest.mark.parametrize("M", [3, 200])
+def test_epilogues(gpu, act, dt, odt, M):
+    for bias, resid in ((False, False), (True, True), (False, True)):
+        _one(M, 320, 192, dt, odt, act, bias, resid, seed=5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,odt", [(BF16, BF16), (BF16, F32), (F32, F32)])
+@pytest.mark.parametrize("M,N,K", [(4, 96, 200), (150, 264, 200), (260, 520, 136)])
+@pytest.mark.parametrize("pad,offset", [((8, 16, 24, 8), 8), ((1, 0, 0, 0), 0), ((0, 3, 0, 0), 0), ((0, 0, 5, 0), 0),
+                                        ((0, 0, 0, 7), 0), ((8, 8, 8, 8), 1), ((5, 7, 9, 11), 3)])
+def test_strides_and_alignment(gpu, M, N, K, pad, offset, dt, odt):
+    _one(M, N, K, dt, odt, "silu", True, True, pad, offset, seed=9)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,odt,M", [(BF16, BF16, 9), (BF16, BF16, 300), (BF16, F32, 300), (F32, F32, 70)])
+def test_out_may_be_the_residual(gpu, dt, odt, M):
+    import torch
+
+    n = _n()
+    N, K = 512, 256
+    x, _ = _rows(torch, M, K, 0, dt, 3)
+    w, _ = _rows(torch, N, K, 0, dt, 4, K ** -0.5)
+    r, _ = _rows(torch, M, N, 8, odt, 5)
+    r0 = r.clone()
+    n.check(_call(n, torch, x, w, dt, odt, "gelu_erf", None, r, r), "linear")
+    torch.cuda.synchronize()
+    _check(torch, r, x, w, None, "gelu_erf", r0, odt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("M", [1, 24, 140])
+def test_values_that_are_not_finite_stay_in_their_rows(gpu, M, dt):
+    import torch
+
+    n = _n()
+    N, K = 264, 136
+    x, _ = _rows(torch, M, K, 0, dt, 3)
+    w, _ = _rows(torch, N, K, 0, dt, 4, 0.1)
+    x[0, 5] = float("inf")
+    if M > 2:
+        x[2, 0] = float("nan")
+    out = torch.zeros(M, N, device="cuda", dtype=_dt(torch, dt))
+    n.check(_call(n, torch, x, w, dt, dt, "relu", None, None, out), "linear")
+    torch.cuda.synchronize()
+    want = torch.where(w[:, 5].float() > 0, float("inf"), 0.0)
+    assert torch.equal(out[0].float(), want)
+    if M > 2:
+        assert torch.isnan(out[2]).all()
+        rest = [i for i in range(M) if i not in (0, 2)]
+        _check(torch, out[rest], x[rest], w, None, "relu", None, dt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,odt", [(BF16, BF16), (F32, F32)])
+def test_captured_on_another_stream_and_replayed(gpu, dt, odt):
+    import torch
+
+    n = _n()
+    for M in (2, 200):
+        N, K = 256, 320
+        x, _ = _rows(torch, M, K, 0, dt, 3)
+        w, _ = _rows(torch, N, K, 0, dt, 4, K ** -0.5)
+        b = torch.randn(N, device="cuda")
+        out = torch.empty(M, N, device="cuda", dtype=_dt(torch, odt))
+        eager = torch.empty_like(out)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(s):
+            n.check(_call(n, torch, x, w, dt, odt, "silu", b, None, eager), "linear")
+        s.synchronize()
+        with torch.cuda.graph(graph, stream=s):
+            st = _call(n, torch, x, w, dt, odt, "silu", b, None, out)
+        n.check(st, "linear")
+        for seed in (7, 8):
+            x.copy_(torch.randn(M, K, generator=torch.Generator().manual_seed(seed)))
+            out.fill_(float("nan"))
+            graph.replay()
+            torch.cuda.synchronize()
+            _check(torch, out, x, w, b, "silu", None, odt)
+        # two calls in flight on two streams, and the same bits each time
+        s2 = torch.cuda.Stream()
+        outs = [torch.empty_like(out) for _ in range(4)]
+        torch.cuda.synchronize()
+        for i, o in enumerate(outs):
+            with torch.cuda.stream(s if i % 2 else s2):
+                n.check(_call(n, torch, x, w, dt, odt, "silu", b, None, o), "linear")
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, out) for o in outs)
+
+
+@pytest.mark.gpu
+def test_memory_the_device_cannot_reach_is_refused(gpu):
+    import torch
+
+    n = _n()
+    x = torch.zeros(2, 8)
+    d = torch.zeros(2, 8, device="cuda")
+    o = torch.zeros(2, 2, device="cuda")
+    for args in ((x, d[:, :8], o), (d, x, o), (d, d, torch.zeros(2, 2))):
+        xx, ww, oo = args
+        assert _call(n, torch, xx, ww, F32, F32, "none", None, None, oo) == INVALID
+        assert "current device" in n.last_error()
+    assert _call(n, torch, d, d, F32, F32, "none", None, None, o) == 0
+    pinned = torch.ones(2, 8).pin_memory()  # pinned host memory is reachable
+    n.check(_call(n, torch, pinned, torch.ones(2, 8, device="cuda"), F32, F32, "none", None, None, o), "linear")
+    torch.cuda.synchronize()
+    assert (o == 8).all()
