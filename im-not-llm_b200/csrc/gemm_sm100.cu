@@ -20,9 +20,11 @@
 // and read W (a few MB) out of L2.
 #include <cstdio>
 #include <cstring>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
+#include "linear.h"
 
 namespace inl {
 
@@ -35,7 +37,7 @@ constexpr int kThreads = 64 + 32 * kEpiWarps;
 
 template <int BN>
 struct GemmCfg {
-  static constexpr int STAGES = BN == 256 ? 4 : 6;
+  static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
   static constexpr int A_BYTES = kBM * kBK * 2;
   static constexpr int B_BYTES = BN * kBK * 2;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
@@ -70,6 +72,10 @@ struct EpiArgs {
   // slices; slice s writes its partial product at out + s * split_stride
   int splits;
   long long split_stride;
+  // linear epilogues
+  const float* bias;
+  int act;
+  int aligned;  // out and resid rows on 16-byte boundaries (bf16: out leaves by TMA), bias on a 16-byte boundary
 };
 
 // A work unit of the persistent schedule: a tile and the K blocks [kb0, kb1)
@@ -160,6 +166,68 @@ __device__ __forceinline__ float ss_bf16_32(const float (&v)[32]) {
     s = fmaf(r.y, r.y, s);
   }
   return s;
+}
+
+// ------------------------------------------------------------------ linear epilogues
+// act(v) of 32 accumulators: one runtime switch per 32 columns instead of a
+// kernel per activation.
+template <typename TO>
+__device__ __forceinline__ void linear_act(float (&v)[32], int act) {
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = f(v[j]);
+  };
+  switch (act) {
+    case INL_ACT_SILU: each([](float x) { return act_for<TO>(x, INL_ACT_SILU); }); break;
+    case INL_ACT_GELU_ERF: each([](float x) { return act_for<TO>(x, INL_ACT_GELU_ERF); }); break;
+    case INL_ACT_GELU_TANH: each([](float x) { return act_for<TO>(x, INL_ACT_GELU_TANH); }); break;
+    case INL_ACT_RELU: each([](float x) { return act_for<TO>(x, INL_ACT_RELU); }); break;
+    case INL_ACT_TANH: each([](float x) { return act_for<TO>(x, INL_ACT_TANH); }); break;
+    default: break;
+  }
+}
+
+// 32 rows x 32 columns of one warp (thread = row, v = its columns) to f32 or
+// unaligned bf16 rows: turned in the warp's 4 KB of shared memory (16-byte
+// piece j of row r at piece j ^ (r & 7): both sides free of bank conflicts) so
+// that neighbouring lanes write, and read the residual at, neighbouring
+// columns, whatever the rows' alignment. row0, col: the chunk's corner.
+template <typename TO, typename TR>
+__device__ __forceinline__ void turn_store32(uint8_t* buf, const float (&v)[32], const EpiArgs& e, TO* out,
+                                             const TR* resid, int row0, int col, int lane) {
+  __syncwarp();  // the chunk before has been read
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    *reinterpret_cast<float4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+        make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  __syncwarp();
+  const int rows = min(32, e.M - row0);
+  if (sizeof(TO) == 4 && e.aligned && e.N - col >= 32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + (lane >> 3), j = lane & 7;
+      if (r >= rows) break;
+      float4 w = *reinterpret_cast<const float4*>(buf + r * 128 + ((j ^ (r & 7)) << 4));
+      if (resid) {
+        const float4 q = *reinterpret_cast<const float4*>(resid + (row0 + r) * e.ldr + col + 4 * j);
+        w.x += q.x, w.y += q.y, w.z += q.z, w.w += q.w;
+      }
+      *reinterpret_cast<float4*>(out + (row0 + r) * e.ldo + col + 4 * j) = w;
+    }
+  } else if (lane < e.N - col) {
+    const int off = lane >> 2;
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r) {
+      float w = *reinterpret_cast<const float*>(buf + r * 128 + ((off ^ (r & 7)) << 4) + (lane & 3) * 4);
+      if constexpr (sizeof(TO) == 4) {
+        if (resid) w += resid[(row0 + r) * e.ldr + col + lane];
+        out[(row0 + r) * e.ldo + col + lane] = w;
+      } else {
+        if (resid) w += __bfloat162float(resid[(row0 + r) * e.ldr + col + lane]);
+        out[(row0 + r) * e.ldo + col + lane] = __float2bfloat16_rn(w);
+      }
+    }
+  }
 }
 
 // One q or k head of width D in TMEM columns [c0, c0 + D) of this thread's row:
@@ -329,6 +397,45 @@ __device__ __forceinline__ void epilogue_tile(uint32_t t_row, int row, int n0, i
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * rs;
           stage_store32(st, v, col + c, row0, lane);
         }
+      }
+    }
+  } else if constexpr (EPI == INL_EPI_LINEAR_BF16 || EPI == INL_EPI_LINEAR_F32) {
+#pragma unroll 1
+    for (int c = 0; c < HW; c += 32) {
+      const int col = n0 + half * HW + c;
+      const int left = e.N - col;
+      if (left <= 0) break;  // warp-uniform
+      tmem_ld32(t_row + half * HW + c, r);
+      if (e.bias == nullptr) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = 0.f;
+      } else if (e.aligned && left >= 32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float4 b = __ldg(reinterpret_cast<const float4*>(e.bias + col) + j);
+          v[4 * j] = b.x, v[4 * j + 1] = b.y, v[4 * j + 2] = b.z, v[4 * j + 3] = b.w;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = j < left ? __ldg(e.bias + col + j) : 0.f;
+      }
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(r[j]);
+      linear_act<std::conditional_t<EPI == INL_EPI_LINEAR_F32, float, __nv_bfloat16>>(v, e.act);
+      if constexpr (EPI == INL_EPI_LINEAR_F32) {
+        turn_store32(st.buf, v, e, static_cast<float*>(e.out), reinterpret_cast<const float*>(e.resid), row0, col,
+                     lane);
+      } else if (e.aligned) {
+        if (e.resid != nullptr && row_ok) {
+          float rr[32];
+          load_row32_bf16(e.resid + static_cast<long long>(row) * e.ldr + col, rr, left);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += rr[j];
+        }
+        stage_store32(st, v, col, row0, lane);
+      } else {
+        turn_store32(st.buf, v, e, static_cast<__nv_bfloat16*>(e.out), e.resid, row0, col, lane);
       }
     }
   } else {
@@ -838,6 +945,16 @@ cudaError_t dispatch_act(int act, const CUtensorMap& ta, const CUtensorMap& tb, 
   }
 }
 
+template <int EPI>
+cudaError_t launch_linear(int bn, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& to, int M, int N,
+                          int K, const EpiArgs& e, int* status, cudaStream_t s) {
+  switch (bn) {
+    case 256: return launch_gemm_pair<EPI, 0>(ta, tb, to, M, N, K, e, status, 0, s);
+    case 128: return launch_gemm<128, EPI, 0>(ta, tb, to, M, N, K, e, status, 0, s);
+    default: return launch_gemm<64, EPI, 0>(ta, tb, to, M, N, K, e, status, 0, s);
+  }
+}
+
 }  // namespace
 
 // Row-major [rows, cols] bf16 with row stride `ld` elements; box [box_rows, box_cols]
@@ -971,6 +1088,50 @@ int gemm_bf16_tn(const GemmArgs& g, cudaStream_t stream) {
       default: return -1;
     }
   }
+  return err == cudaSuccess ? 0 : -3;
+}
+
+bool gemm_bf16_linear_takes(const GemmArgs& g) {
+  // what a TMA map asks of x and w: 16-byte rows (K may end anywhere inside one)
+  auto rows_ok = [](const void* p, long long ld, long long rows) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (rows == 1 || (ld % 8 == 0 && ld * 2 < (1ll << 40)));
+  };
+  return g.K > 0 && rows_ok(g.A, g.lda, g.M) && rows_ok(g.W, g.ldw, g.N);
+}
+
+int gemm_bf16_linear(const GemmArgs& g, bool out_bf16, cudaStream_t stream) {
+  if (g.M <= 0 || g.N <= 0 || !gemm_bf16_linear_takes(g)) return -1;
+  auto pad8 = [](long long n) { return (n + 7) & ~7ll; };
+  const long long lda = g.M == 1 ? pad8(g.K) : g.lda, ldw = g.N == 1 ? pad8(g.K) : g.ldw;
+  EpiArgs e{};
+  e.out = g.out, e.ldo = g.ldo, e.resid = g.resid, e.ldr = g.ldr, e.status = g.status, e.M = g.M, e.N = g.N;
+  e.splits = 1, e.bias = g.bias, e.act = g.act;
+  const int per16 = out_bf16 ? 8 : 4;
+  auto on16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  auto ld_ok = [&](long long ld) { return g.M == 1 || (ld % per16 == 0 && ld * (16 / per16) < (1ll << 40)); };
+  e.aligned = on16(g.out) && ld_ok(g.ldo) && (!g.resid || (on16(g.resid) && ld_ok(g.ldr))) && on16(g.bias);
+  // The tile that finishes first by (waves over the SMs) x (time of a tile): at
+  // K = 1024 a 256 x 256 tile of a CTA pair takes 7.2 us, a 128 x 128 tile 5.0,
+  // a 128 x 64 tile 4.6 in a long run, and 8 : 6 : 5 where there is one wave.
+  // Measured (us), pair / 128 / 64: 1024 x 1024 x 1024 11.2 / 8.7 / 8.1;
+  // 2048 x 1024 x 1024 11.4 / 8.9 / 12.8; 1024 x 4096 x 1024 12.2 / 14.2 / 22.1;
+  // 8192 x 1024 x 2048 28.9 / 40.8 / 65.4.
+  const long long sms = num_sms();
+  auto waves = [&](long long bm, long long bn, long long at_once) {
+    return ((g.M + bm - 1) / bm * ((g.N + bn - 1) / bn) + at_once - 1) / at_once;
+  };
+  const long long t256 = 8 * waves(256, 256, sms / 2), t128 = 6 * waves(128, 128, sms), t64 = 5 * waves(128, 64, sms);
+  const int bn = t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64;
+  CUtensorMap ta, tb, to;
+  if (!make_kmajor_map(&ta, g.A, g.M, g.K, lda, kBM)) return -2;
+  if (!make_kmajor_map(&tb, g.W, g.N, g.K, ldw, bn == 256 ? 128 : bn)) return -2;
+  std::memset(&to, 0, sizeof(to));
+  if (out_bf16 && e.aligned &&
+      !make_tma_2d_bf16_swizzled(&to, g.out, g.M, g.N, g.M == 1 ? pad8(g.N) : g.ldo, 32, 32, 64))
+    return -2;
+  const cudaError_t err =
+      out_bf16 ? launch_linear<INL_EPI_LINEAR_BF16>(bn, ta, tb, to, g.M, g.N, g.K, e, g.status, stream)
+               : launch_linear<INL_EPI_LINEAR_F32>(bn, ta, tb, to, g.M, g.N, g.K, e, g.status, stream);
   return err == cudaSuccess ? 0 : -3;
 }
 

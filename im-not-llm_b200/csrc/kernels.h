@@ -23,12 +23,21 @@ enum InlEpilogue : int {
   INL_EPI_SEGMAX = 5,      // pooled[seg[col]][row] = max over columns of the segment (order-encoded atomicMax)
   INL_EPI_RESID_F32 = 6,   // out = r * acc + resid, f32 (resid read as f32; out may alias resid)
   INL_EPI_GATED_F32 = 7,   // as INL_EPI_GATED_BF16 with an f32 output
+  INL_EPI_LINEAR_BF16 = 8, // out = bf16(act(r * acc + bias) + resid); bias and resid (bf16) may be null
+  INL_EPI_LINEAR_F32 = 9,  // the same with an f32 output and residual
 };
 
 // Columns per partial sum of squares written by the residual epilogue.
 constexpr int INL_SS_COLS = 64;
 
-enum InlAct : int { INL_ACT_SILU = 0, INL_ACT_GELU_ERF = 1, INL_ACT_GELU_TANH = 2 };
+enum InlAct : int {
+  INL_ACT_SILU = 0,
+  INL_ACT_GELU_ERF = 1,
+  INL_ACT_GELU_TANH = 2,
+  INL_ACT_NONE = 3,  // 3 to 5: the linear epilogues only
+  INL_ACT_RELU = 4,
+  INL_ACT_TANH = 5,
+};
 
 namespace inl {
 
@@ -72,10 +81,18 @@ struct GemmArgs {
   // split-K (INL_EPI_F32 only): each tile's K blocks in `splits` slices, slice
   // s writing its partial product to out + s * M * ldo (splits_reduce_f32 sums them)
   int splits = 1;
+  // linear epilogues: [N] f32 or null (resid, ldr above: the output's type)
+  const float* bias = nullptr;
 };
 
 // tcgen05 bf16 GEMM; returns 0 on success, <0 on bad arguments / launch error.
 int gemm_bf16_tn(const GemmArgs& g, cudaStream_t stream);
+
+// out = act(A W^T + bias) + resid on the same kernels (out and resid bf16 or
+// f32 of any alignment). `takes`: whether A and W have the 16-byte rows of a
+// TMA load; K may be any positive number.
+bool gemm_bf16_linear_takes(const GemmArgs& g);
+int gemm_bf16_linear(const GemmArgs& g, bool out_bf16, cudaStream_t stream);
 
 // 2D TMA descriptor of a row-major bf16 matrix, 128-byte swizzle, box [box_rows, box_cols].
 bool make_tma_2d_bf16(CUtensorMap* map, const void* base, long long rows, long long cols, long long ld,

@@ -12,43 +12,11 @@
 #include "common.cuh"
 #include "hook_checks.h"
 #include "kernels.h"
+#include "linear.h"
 
 namespace inl {
 
 namespace {
-
-struct LinearArgs {
-  const void* x;
-  const void* w;
-  const float* bias;
-  const void* resid;
-  void* out;
-  long long ldx, ldw, ldr, ldo;
-  int M, N, K, act;
-};
-
-template <typename T>
-__device__ __forceinline__ float load_f(const T* p) {
-  if constexpr (sizeof(T) == 2) return __bfloat162float(*p);
-  else return *p;
-}
-template <typename T>
-__device__ __forceinline__ void store_f(T* p, float v) {
-  if constexpr (sizeof(T) == 2) *p = __float2bfloat16_rn(v);
-  else *p = v;
-}
-
-// Activations to f32 accuracy.
-__device__ __forceinline__ float act_exact(float v, int act) {
-  switch (act) {
-    case INL_ACT_SILU_: return v / (1.0f + expf(-v));
-    case INL_ACT_GELU_ERF_: return gelu_erf_f(v);
-    case INL_ACT_GELU_TANH_: return gelu_tanh_f(v);
-    case INL_ACT_RELU_: return v < 0.f ? 0.f : v;  // NaN stays
-    case INL_ACT_TANH_: return tanhf(v);
-    default: return v;
-  }
-}
 
 template <typename TX, typename TO>
 __global__ void __launch_bounds__(256) linear_any_kernel(LinearArgs g) {
@@ -109,12 +77,27 @@ cudaError_t launch_linear_any(const LinearArgs& g, cudaStream_t s) {
 
 int bad(const char* why) { return record_error(INL_ERR_INVALID_INPUT, std::string("linear: ") + why); }
 
+// CTAs per cluster for a product whose 128 x 64 tiles leave SMs idle: 4 or 2
+// while all of them run at once and each keeps 4 (or 3) blocks of 64 k. An SM
+// takes operands from L2 at about 100 KB/us, so a lone CTA needs 0.24 us per
+// block of k. Measured (us), S = 1 (the persistent kernel) / 2 / 4:
+// 128 x 1024 x 1024 7.6 / 6.4 / 6.1; 256 x 768 x 768 6.5 / 5.9 / 6.2;
+// 256 x 1024 x 2048 11.9 / 8.7 / 8.0; 512 x 1024 x 2048 12.2 / 9.2 / 15.6;
+// 64 x 4096 x 1024 7.7 / 6.5 / 12.7. S = 8 took 11 us and more.
+int cluster_size(const LinearArgs& g, int sms) {
+  const long long tiles = static_cast<long long>((g.M + 127) / 128) * ((g.N + 63) / 64);
+  const int k_blocks = (g.K + 63) / 64;
+  if (tiles * 4 <= sms && k_blocks >= 16) return 4;
+  return tiles * 2 <= sms && k_blocks >= 6 ? 2 : 1;
+}
+
 int linear(const LinearArgs& g, int dtype, int out_dtype, int* status, cudaStream_t s) {
   if ((dtype != INL_DTYPE_F32 && dtype != INL_DTYPE_BF16) || (out_dtype != INL_DTYPE_F32 && out_dtype != INL_DTYPE_BF16))
     return bad("dtypes are f32 or bf16");
   constexpr int kMost = 1 << 30;  // tile indices and K offsets stay in 32 bits
   if (g.M < 0 || g.N < 0 || g.K < 0 || g.M > kMost || g.N > kMost || g.K > kMost)
     return bad("M, N, K from 0 to 2^30");
+  if (static_cast<long long>(g.M) * g.N > (1ll << 40)) return bad("M * N at most 2^40");
   if (g.act < INL_ACT_SILU_ || g.act > INL_ACT_TANH_) return bad("unknown activation");
   if (g.M == 0 || g.N == 0) return INL_OK;
   for (long long ld : {g.ldx, g.ldw, g.ldr, g.ldo})
@@ -130,6 +113,21 @@ int linear(const LinearArgs& g, int dtype, int out_dtype, int* status, cudaStrea
   int r;
   if ((r = check_aligned("linear", ptrs)) || (r = check_reachable("linear", ptrs))) return r;
   const bool xb = dtype == INL_DTYPE_BF16, ob = out_dtype == INL_DTYPE_BF16;
+  GemmArgs t;
+  t.A = static_cast<const __nv_bfloat16*>(g.x), t.lda = g.ldx;
+  t.W = static_cast<const __nv_bfloat16*>(g.w), t.ldw = g.ldw;
+  t.M = g.M, t.N = g.N, t.K = g.K, t.act = g.act, t.bias = g.bias;
+  t.out = g.out, t.ldo = g.ldo, t.resid = static_cast<const __nv_bfloat16*>(g.resid), t.ldr = g.ldr;
+  t.status = status;
+  if (xb && gemm_bf16_linear_takes(t)) {
+    const int sms = num_sms_cached();
+    if (g.M <= 32 || (g.M <= 64 && g.N <= 8 * sms)) return launched("linear", linear_skinny(g, ob, s));
+    const int S = cluster_size(g, sms);
+    if (S > 1) return launched("linear", linear_cluster(g, ob, S, status, s));
+    const int rc = gemm_bf16_linear(t, ob, s);
+    if (rc == 0) return INL_OK;
+    return record_error(INL_ERR_INFERENCE, rc == -3 ? "linear launch failed" : "linear: no TMA map for x, w or out");
+  }
   return launched("linear", xb ? (ob ? launch_linear_any<__nv_bfloat16, __nv_bfloat16>(g, s)
                                      : launch_linear_any<__nv_bfloat16, float>(g, s))
                                : (ob ? launch_linear_any<float, __nv_bfloat16>(g, s)

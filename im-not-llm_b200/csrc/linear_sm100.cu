@@ -1,0 +1,341 @@
+// Linear layers of few rows, out = act(x w^T + bias) + resid with bf16 operands:
+// the sizes at which the persistent GEMM leaves most of the SMs idle.
+//
+// linear_skinny_kernel: up to 64 rows. The product is a read of w, so w goes
+// from global memory straight into mma.sync fragments, with no shared memory
+// in between: the k order inside a product is free as long as x and w agree, so
+// a lane takes 16 contiguous bytes of its row as the k pairs (0,1 | 8,9) of one
+// m16n8k16 and of the next. A CTA owns 8 NT rows of w, its 8 warps split K and
+// are summed in shared memory in warp order.
+//
+// linear_cluster_kernel: some hundreds of rows, or few columns. A cluster of S
+// CTAs shares one 128 x 64 tile, each with its own slice of K on tcgen05
+// (TMA ring, accumulator in TMEM); the partial tiles meet in shared memory and
+// every CTA sums its share of the elements over the cluster's copies, in rank
+// order, and runs the epilogue on it. No workspace, no atomics, the same bits
+// every time.
+#include <algorithm>
+
+#include "../../include/inl_cuda.h"
+#include "../../include/inl_cuda_kernels.h"
+#include "common.cuh"
+#include "kernels.h"
+#include "linear.h"
+
+namespace inl {
+
+namespace {
+
+// ------------------------------------------------------------------ skinny
+__device__ __forceinline__ void mma_bf16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 8 bf16 of a row from element k on, zero past K (the row's last piece is
+// read element by element: nothing past K is touched).
+__device__ __forceinline__ uint4 load8_to(const __nv_bfloat16* row, int k, int K) {
+  if (K - k >= 8) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  uint32_t h[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) h[i] = k + i < K ? reinterpret_cast<const uint16_t*>(row)[k + i] : 0u;
+  return make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+}
+
+template <typename TO, int MT, int NT, int U, int W>
+__global__ void __launch_bounds__(32 * W) linear_skinny_kernel(LinearArgs g) {
+  extern __shared__ float red_raw[];
+  auto red = reinterpret_cast<float(*)[MT * 16][NT * 8 + 1]>(red_raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n0 = blockIdx.x * NT * 8;
+  const int r = lane >> 2, kq = (lane & 3) * 8;
+  const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(g.x);
+  const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(g.w);
+  float acc[MT][NT][4] = {};
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  for (int k0 = warp * 32; k0 < g.K; k0 += W * 32 * U) {
+    uint4 wv[U][NT], xv[U][MT][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * W * 32 + kq;
+      const bool k_ok = k < g.K;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int n = n0 + j * 8 + r;
+        wv[u][j] = k_ok && n < g.N ? load8_to(w + n * g.ldw, k, g.K) : zero;
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const int m = i * 16 + r;
+        xv[u][i][0] = k_ok && m < g.M ? load8_to(x + m * g.ldx, k, g.K) : zero;
+        xv[u][i][1] = k_ok && m + 8 < g.M ? load8_to(x + (m + 8) * g.ldx, k, g.K) : zero;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const uint4 lo = xv[u][i][0], hi = xv[u][i][1];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          mma_bf16_16816(acc[i][j], lo.x, hi.x, lo.y, hi.y, wv[u][j].x, wv[u][j].y);
+          mma_bf16_16816(acc[i][j], lo.z, hi.z, lo.w, hi.w, wv[u][j].z, wv[u][j].w);
+        }
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) red[warp][i * 16 + r + (e >> 1) * 8][j * 8 + (lane & 3) * 2 + (e & 1)] = acc[i][j][e];
+  __syncthreads();
+  for (int o = threadIdx.x; o < MT * 16 * NT * 8; o += 32 * W) {
+    const int m = o / (NT * 8), c = o % (NT * 8), n = n0 + c;
+    if (m >= g.M || n >= g.N) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int s = 0; s < W; ++s) v += red[s][m][c];
+    linear_finish(g, v, static_cast<long long>(m), n, static_cast<TO*>(g.out));
+  }
+}
+
+template <typename TO, int MT, int NT, int U, int W>
+cudaError_t launch_skinny(const LinearArgs& g, cudaStream_t s) {
+  linear_skinny_kernel<TO, MT, NT, U, W><<<(g.N + 8 * NT - 1) / (8 * NT), 32 * W, W * MT * 16 * (NT * 8 + 1) * 4, s>>>(g);
+  return cudaGetLastError();
+}
+
+template <typename TO>
+cudaError_t launch_skinny_for(const LinearArgs& g, cudaStream_t s) {
+  // Few columns: 8 rows of w per CTA, on as many SMs as that gives. More: more
+  // rows of w per CTA, so that each load of x serves them all, while about two
+  // CTAs of 8 warps stay on each SM; 16 warps where an SM has one CTA.
+  // Measured (us), 8 / 16 / 32 rows of w per CTA: M = 1, K = 1024: N = 1024
+  // 2.8 / 2.8 / 3.5, N = 4096 5.1 / 3.2 / 3.5; M = 16, K = 768, N = 2304
+  // 3.3 / 3.0 / 3.6; M = 32, K = 1024, N = 4096 6.5 / 6.8 / 5.9. 16 against 8
+  // warps: M = 1, N = K = 1024 2.6 / 2.8; M = 19, N = 1024, K = 2048 4.1 / 4.7;
+  // M = 1, N = 2048, K = 2048 (256 CTAs) 4.9 / 3.6.
+  const int sms = num_sms_cached();
+  const bool one = g.N <= 8 * sms;
+  if (g.M <= 16) {
+    if (one) return launch_skinny<TO, 1, 1, 4, 16>(g, s);
+    if (g.N <= 14 * sms) return launch_skinny<TO, 1, 1, 8, 8>(g, s);
+    if (g.N <= 28 * sms) return launch_skinny<TO, 1, 2, 4, 8>(g, s);
+    return launch_skinny<TO, 1, 4, 4, 8>(g, s);
+  }
+  if (g.M <= 32) {
+    if (one) return launch_skinny<TO, 2, 1, 4, 16>(g, s);
+    if (g.N <= 14 * sms) return launch_skinny<TO, 2, 1, 4, 8>(g, s);
+    return launch_skinny<TO, 2, 4, 2, 8>(g, s);
+  }
+  return launch_skinny<TO, 4, 1, 2, 16>(g, s);
+}
+
+// ------------------------------------------------------------------ cluster split-K
+constexpr int kBM = 128, kBK = 64;
+constexpr int kBN = 64;
+constexpr int kThreads = 320;  // warp 0 TMA, warp 1 MMA, warps 2..9 move the accumulator out
+
+struct ClusterCfg {
+  static constexpr int STAGES = 6;
+  static constexpr int A_BYTES = kBM * kBK * 2, B_BYTES = kBN * kBK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int PART_BYTES = kBM * kBN * 4;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + PART_BYTES + 1024 + 256;
+};
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr));
+  return v;
+}
+
+template <typename TO>
+__global__ void __launch_bounds__(kThreads, 1)
+    linear_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                          LinearArgs g, int S, int wide, int* status) {
+  using C = ClusterCfg;
+  constexpr int BN = kBN;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + C::STAGES * C::A_BYTES;
+  uint8_t* part = sB + C::STAGES * C::B_BYTES;  // this CTA's partial tile, f32
+  uint64_t* full = reinterpret_cast<uint64_t*>(part + C::PART_BYTES);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* tfull = empty + C::STAGES;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tfull + 1);
+
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int tile = blockIdx.x / S;
+  const int n_tiles = (g.N + BN - 1) / BN;
+  const int m0 = tile / n_tiles * kBM, n0 = tile % n_tiles * BN;
+  const int k_blocks = (g.K + kBK - 1) / kBK;
+  const int kb0 = k_blocks * rank / S, kb1 = k_blocks * (rank + 1) / S;  // at least one block each (S <= k_blocks)
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(tfull, 1);
+    fence_barrier_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_holder, BN);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  pdl_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int issued = 0;
+      for (int kb = kb0; kb < kb1; ++kb, ++issued) {
+        const int st = issued % C::STAGES;
+        if (!mbar_wait(&empty[st], ((issued / C::STAGES) & 1) ^ 1, status, INL_DEV_TIMEOUT_PRODUCER)) break;
+        mbar_expect_tx(&full[st], C::STAGE_BYTES);
+        tma_load_2d(sA + st * C::A_BYTES, &tmA, &full[st], kb * kBK, m0);
+        tma_load_2d(sB + st * C::B_BYTES, &tmB, &full[st], kb * kBK, n0);
+      }
+      // every copy has landed before the CTA can leave
+      for (int f = max(0, issued - C::STAGES); f < issued; ++f)
+        if (!mbar_wait(&full[f % C::STAGES], (f / C::STAGES) & 1, status, INL_DEV_TIMEOUT_DRAIN)) break;
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = umma_idesc_bf16(kBM, BN);
+      bool ok = true;
+      for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
+        const int st = i % C::STAGES;
+        if (!(ok = mbar_wait(&full[st], (i / C::STAGES) & 1, status, INL_DEV_TIMEOUT_MMA))) break;
+        tc_fence_after();
+        const uint64_t a = sw128_kmajor_desc(smem_u32(sA + st * C::A_BYTES));
+        const uint64_t b = sw128_kmajor_desc(smem_u32(sB + st * C::B_BYTES));
+#pragma unroll
+        for (int kk = 0; kk < kBK / 16; ++kk)
+          umma_bf16(tmem, a + static_cast<uint64_t>(kk * 2), b + static_cast<uint64_t>(kk * 2), idesc,
+                    (i != 0 || kk != 0) ? 1u : 0u);
+        umma_commit(&empty[st]);
+      }
+      if (ok) umma_commit(tfull);
+    }
+  } else {
+    // thread = tile row; 16-byte piece j of a 32-column group at j ^ (row & 7)
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    if (mbar_wait_warp(tfull, 0, status, INL_DEV_TIMEOUT_EPILOGUE)) {
+      tc_fence_after();
+      const int row = quad * 32 + lane;
+      if (m0 + quad * 32 < g.M) {  // warp-uniform
+#pragma unroll 1
+        for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
+          uint32_t v[32];
+          tmem_ld32(tmem + (static_cast<uint32_t>(quad * 32) << 16) + c, v);
+          tmem_ld_wait();
+          uint8_t* dst = part + row * (BN * 4) + c * 4;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4*>(dst + ((j ^ (row & 7)) << 4)) =
+                make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  cluster_sync_all();  // every partial tile is written
+  // A thread keeps one 4-column piece; the cluster's CTAs take its rows in turn,
+  // four rows (4 S loads) in flight at a time.
+  constexpr int Q = BN / 4, STEP = 256 / Q;
+  if (warp >= 2) {
+    const int tid = threadIdx.x - 64, q = tid % Q, n = n0 + 4 * q;
+    const int rows = min(kBM, g.M - m0);
+    if (n < g.N) {
+      float bias[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bias[i] = g.bias && n + i < g.N ? __ldg(g.bias + n + i) : 0.f;
+      const uint32_t col = smem_u32(part) + (q >> 3) * 128;
+      for (int r0 = rank * STEP + tid / Q; r0 < rows; r0 += 4 * S * STEP) {
+        float4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = make_float4(bias[0], bias[1], bias[2], bias[3]);
+        for (int s = 0; s < S; ++s) {
+          const uint32_t base = mapa_shared(col, s);
+          float4 p[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = min(r0 + i * S * STEP, rows - 1);
+            p[i] = ld_cluster_f4(base + row * (BN * 4) + (((q & 7) ^ (row & 7)) << 4));
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i].x += p[i].x, v[i].y += p[i].y, v[i].z += p[i].z, v[i].w += p[i].w;
+        }
+        linear_finish_rows<TO, 4>(g, v, m0 + r0, S * STEP, min(4, (rows - r0 + S * STEP - 1) / (S * STEP)), n, wide);
+      }
+    }
+  }
+  cluster_sync_all();  // no CTA leaves while another may still read its partial tile
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, BN);
+  }
+}
+
+template <typename TO>
+cudaError_t launch_cluster(const CUtensorMap& ta, const CUtensorMap& tb, const LinearArgs& g, int S, int wide,
+                           int* status, cudaStream_t s) {
+  using C = ClusterCfg;
+  auto kern = linear_cluster_kernel<TO>;
+  static std::atomic<unsigned long long> attr_set{0};
+  cudaError_t err = set_smem_limit_once(kern, C::SMEM_BYTES, attr_set);
+  if (err != cudaSuccess) return err;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(((g.M + kBM - 1) / kBM) * ((g.N + kBN - 1) / kBN) * S);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::SMEM_BYTES;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = S;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kern, ta, tb, g, S, wide, status);
+}
+
+}  // namespace
+
+cudaError_t linear_skinny(const LinearArgs& g, bool out_bf16, cudaStream_t s) {
+  return out_bf16 ? launch_skinny_for<__nv_bfloat16>(g, s) : launch_skinny_for<float>(g, s);
+}
+
+cudaError_t linear_cluster(const LinearArgs& g, bool out_bf16, int S, int* status, cudaStream_t s) {
+  auto pad8 = [](long long n) { return (n + 7) & ~7ll; };
+  CUtensorMap ta, tb;
+  if (!make_tma_2d_bf16(&ta, g.x, g.M, g.K, g.M == 1 ? pad8(g.K) : g.ldx, kBM, kBK) ||
+      !make_tma_2d_bf16(&tb, g.w, g.N, g.K, g.N == 1 ? pad8(g.K) : g.ldw, kBN, kBK))
+    return cudaErrorInvalidValue;
+  // 4 columns in one access: rows of out and resid on its boundary
+  const int bytes = out_bf16 ? 8 : 16;
+  auto ok = [&](const void* p, long long ld) {
+    return (reinterpret_cast<uintptr_t>(p) % bytes) == 0 && (g.M == 1 || ld % 4 == 0);
+  };
+  const int wide = ok(g.out, g.ldo) && (!g.resid || ok(g.resid, g.ldr));
+  return out_bf16 ? launch_cluster<__nv_bfloat16>(ta, tb, g, S, wide, status, s)
+                  : launch_cluster<float>(ta, tb, g, S, wide, status, s);
+}
+
+}  // namespace inl
