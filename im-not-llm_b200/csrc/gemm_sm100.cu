@@ -991,6 +991,19 @@ bool make_tma_2d_bf16(CUtensorMap* map, const void* base, long long rows, long l
   return r == CUDA_SUCCESS;
 }
 
+bool make_tma_2d_f32(CUtensorMap* map, const void* base, long long rows, long long cols, long long ld, int box_rows,
+                     int box_cols) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 4};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int num_sms_cached() { return num_sms(); }
 
 int gemm_bf16_tn(const GemmArgs& g, cudaStream_t stream) {

@@ -97,6 +97,9 @@ int gemm_bf16_linear(const GemmArgs& g, bool out_bf16, cudaStream_t stream);
 // 2D TMA descriptor of a row-major bf16 matrix, 128-byte swizzle, box [box_rows, box_cols].
 bool make_tma_2d_bf16(CUtensorMap* map, const void* base, long long rows, long long cols, long long ld,
                       int box_rows, int box_cols);
+// The same of f32 (box_cols 32).
+bool make_tma_2d_f32(CUtensorMap* map, const void* base, long long rows, long long cols, long long ld, int box_rows,
+                     int box_cols);
 int num_sms_cached();
 
 // Raises a kernel's dynamic shared-memory limit on the current device, once

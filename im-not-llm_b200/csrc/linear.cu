@@ -91,6 +91,23 @@ int cluster_size(const LinearArgs& g, int sms) {
   return tiles * 2 <= sms && k_blocks >= 6 ? 2 : 1;
 }
 
+// The same for the f32 kernel, whose CTAs take one tile each: the S of the
+// least (waves over the SMs) x (blocks of 32 k + 4 for a tile's start and end).
+// Measured (us), S = 1 / 2 / 4 / 8: 1024 x 1024 x 1024 36 / 21 / 29 / 74;
+// 1024 x 4096 x 1024 72 / 85 / 117 / 262; 8192 x 1024 x 4096 478 / 444 / 575 /
+// 906; 4253 x 768 x 768 66 / 58 / 94 / 201; 32 x 1024 x 1024 40 / 22 / 15 / 12.
+int f32_cluster_size(const LinearArgs& g, int sms) {
+  const long long tiles = static_cast<long long>((g.M + 127) / 128) * ((g.N + 127) / 128);
+  const int k_blocks = (g.K + 31) / 32;
+  int best = 1;
+  long long least = -1;
+  for (int S = 1; S <= 8 && S <= k_blocks; S *= 2) {
+    const long long cost = (tiles * S + sms - 1) / sms * ((k_blocks + S - 1) / S + 4);
+    if (least < 0 || cost < least) least = cost, best = S;
+  }
+  return best;
+}
+
 int linear(const LinearArgs& g, int dtype, int out_dtype, int* status, cudaStream_t s) {
   if ((dtype != INL_DTYPE_F32 && dtype != INL_DTYPE_BF16) || (out_dtype != INL_DTYPE_F32 && out_dtype != INL_DTYPE_BF16))
     return bad("dtypes are f32 or bf16");
@@ -119,8 +136,8 @@ int linear(const LinearArgs& g, int dtype, int out_dtype, int* status, cudaStrea
   t.M = g.M, t.N = g.N, t.K = g.K, t.act = g.act, t.bias = g.bias;
   t.out = g.out, t.ldo = g.ldo, t.resid = static_cast<const __nv_bfloat16*>(g.resid), t.ldr = g.ldr;
   t.status = status;
+  const int sms = num_sms_cached();
   if (xb && gemm_bf16_linear_takes(t)) {
-    const int sms = num_sms_cached();
     if (g.M <= 32 || (g.M <= 64 && g.N <= 8 * sms)) return launched("linear", linear_skinny(g, ob, s));
     const int S = cluster_size(g, sms);
     if (S > 1) return launched("linear", linear_cluster(g, ob, S, status, s));
@@ -128,6 +145,7 @@ int linear(const LinearArgs& g, int dtype, int out_dtype, int* status, cudaStrea
     if (rc == 0) return INL_OK;
     return record_error(INL_ERR_INFERENCE, rc == -3 ? "linear launch failed" : "linear: no TMA map for x, w or out");
   }
+  if (!xb && linear_f32_takes(g)) return launched("linear", linear_f32(g, ob, f32_cluster_size(g, sms), status, s));
   return launched("linear", xb ? (ob ? launch_linear_any<__nv_bfloat16, __nv_bfloat16>(g, s)
                                      : launch_linear_any<__nv_bfloat16, float>(g, s))
                                : (ob ? launch_linear_any<float, __nv_bfloat16>(g, s)

@@ -2,6 +2,8 @@
 // (linear.cu, linear_sm100.cu).
 #pragma once
 
+#include <utility>
+
 #include "../../include/inl_cuda_kernels.h"
 #include "common.cuh"
 
@@ -157,10 +159,117 @@ __device__ __forceinline__ void linear_finish_rows(const LinearArgs& g, float4 (
   }
 }
 
+// ------------------------------------------------------------------ clusters that share out K
+// Each CTA's partial tile [128, BN] f32 in its shared memory: 16-byte piece q of
+// a row at q ^ (row & 7) inside its 128-byte group, so that a warp writing 32
+// rows of one piece and one reading a row's pieces both miss bank conflicts.
+template <int BN>
+__device__ __forceinline__ uint8_t* cluster_piece(uint8_t* part, int row, int q) {
+  return part + row * (BN * 4) + (q >> 3) * 128 + (((q & 7) ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr));
+  return v;
+}
+// A plain f32 sum, ended by the first NaN.
+__device__ __forceinline__ float plain_dot(const LinearArgs& g, long long m, long long n) {
+  const float* x = static_cast<const float*>(g.x) + m * g.ldx;
+  const float* w = static_cast<const float*>(g.w) + n * g.ldw;
+  float s = 0.f;
+  for (int k = 0; k < g.K && !isnan(s); ++k) s = fmaf(x[k], w[k], s);
+  return s;
+}
+
+// After a cluster barrier: 256 threads (tid) of each of the S CTAs sum their
+// share of the tile over the cluster's partial tiles, in rank order, and run
+// the epilogue on it. A thread keeps one 4-column piece; the CTAs take its rows
+// in turn, four rows (4 S loads) in flight at a time. REDO: a NaN is computed
+// again as a plain f32 sum.
+template <typename TO, int BN, bool REDO>
+__device__ __forceinline__ void cluster_finish(const LinearArgs& g, uint8_t* part, int tid, int rank, int S, int m0,
+                                               int n0, bool wide) {
+  constexpr int Q = BN / 4, STEP = 256 / Q;
+  const int q = tid % Q, n = n0 + 4 * q, rows = min(128, g.M - m0);
+  if (n >= g.N) return;
+  float bias[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bias[i] = g.bias && n + i < g.N ? __ldg(g.bias + n + i) : 0.f;
+  const uint32_t mine = smem_u32(part);
+  for (int r0 = rank * STEP + tid / Q; r0 < rows; r0 += 4 * S * STEP) {
+    float4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < S; ++s) {
+      const uint32_t base = mapa_shared(mine, s);
+      float4 p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = min(r0 + i * S * STEP, rows - 1);
+        p[i] = ld_cluster_f4(base + static_cast<uint32_t>(cluster_piece<BN>(part, row, q) - part));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i].x += p[i].x, v[i].y += p[i].y, v[i].z += p[i].z, v[i].w += p[i].w;
+    }
+    const int count = min(4, (rows - r0 + S * STEP - 1) / (S * STEP));
+    if constexpr (REDO) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i >= count || !isnan(v[i].x + v[i].y + v[i].z + v[i].w)) continue;
+        const long long m = m0 + r0 + i * S * STEP;
+        if (isnan(v[i].x)) v[i].x = plain_dot(g, m, n);
+        if (isnan(v[i].y) && n + 1 < g.N) v[i].y = plain_dot(g, m, n + 1);
+        if (isnan(v[i].z) && n + 2 < g.N) v[i].z = plain_dot(g, m, n + 2);
+        if (isnan(v[i].w) && n + 3 < g.N) v[i].w = plain_dot(g, m, n + 3);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i].x += bias[0], v[i].y += bias[1], v[i].z += bias[2], v[i].w += bias[3];
+    linear_finish_rows<TO, 4>(g, v, m0 + r0, S * STEP, count, n, wide);
+  }
+}
+
+// Whether rows of out and resid take 4 columns in one access.
+inline int linear_wide(const LinearArgs& g, bool out_bf16) {
+  const uintptr_t bytes = out_bf16 ? 8 : 16;
+  auto ok = [&](const void* p, long long ld) {
+    return (reinterpret_cast<uintptr_t>(p) % bytes) == 0 && (g.M == 1 || ld % 4 == 0);
+  };
+  return ok(g.out, g.ldo) && (!g.resid || ok(g.resid, g.ldr));
+}
+
+// A launch in clusters of S CTAs, allowed to start while its predecessor ends
+// (launch_pdl).
+template <typename... Params, typename... Args>
+cudaError_t launch_cluster_pdl(void (*kern)(Params...), unsigned grid, int threads, size_t smem, int S, cudaStream_t s,
+                               Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = S;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
 // linear_sm100.cu. Both want 16-byte rows of x and w (gemm_bf16_linear_takes).
 // At most 64 rows.
 cudaError_t linear_skinny(const LinearArgs& g, bool out_bf16, cudaStream_t s);
 // Clusters of S CTAs (1 to 8, at most ceil(K / 64)) split K.
 cudaError_t linear_cluster(const LinearArgs& g, bool out_bf16, int S, int* status, cudaStream_t s);
+
+// linear_f32_sm100.cu: f32 operands; `takes`: 16-byte rows of x and w. S from 1
+// to 8, at most ceil(K / 32).
+bool linear_f32_takes(const LinearArgs& g);
+cudaError_t linear_f32(const LinearArgs& g, bool out_bf16, int S, int* status, cudaStream_t s);
 
 }  // namespace inl

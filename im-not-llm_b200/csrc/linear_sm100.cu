@@ -142,18 +142,11 @@ constexpr int kThreads = 320;  // warp 0 TMA, warp 1 MMA, warps 2..9 move the ac
 
 struct ClusterCfg {
   static constexpr int STAGES = 6;
+  static constexpr int CHUNK = 8;  // K blocks (512 of K) between promotions of the sum
   static constexpr int A_BYTES = kBM * kBK * 2, B_BYTES = kBN * kBK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int PART_BYTES = kBM * kBN * 4;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + PART_BYTES + 1024 + 256;
 };
-
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr));
-  return v;
-}
 
 template <typename TO>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -169,7 +162,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* full = reinterpret_cast<uint64_t*>(part + C::PART_BYTES);
   uint64_t* empty = full + C::STAGES;
   uint64_t* tfull = empty + C::STAGES;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tfull + 1);
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tempty + 2);
 
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -178,20 +172,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int n_tiles = (g.N + BN - 1) / BN;
   const int m0 = tile / n_tiles * kBM, n0 = tile % n_tiles * BN;
   const int k_blocks = (g.K + kBK - 1) / kBK;
-  const int kb0 = k_blocks * rank / S, kb1 = k_blocks * (rank + 1) / S;  // at least one block each (S <= k_blocks)
+  const int kb0 = static_cast<int>(static_cast<long long>(k_blocks) * rank / S);
+  const int nkb = static_cast<int>(static_cast<long long>(k_blocks) * (rank + 1) / S) - kb0;  // > 0: S <= k_blocks
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(tfull, 1);
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], 8);
+    }
     fence_barrier_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_holder, BN);
+    tmem_alloc(tmem_holder, 2 * BN);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -203,8 +201,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     if (lane == 0) {
       int issued = 0;
-      for (int kb = kb0; kb < kb1; ++kb, ++issued) {
-        const int st = issued % C::STAGES;
+      for (; issued < nkb; ++issued) {
+        const int st = issued % C::STAGES, kb = kb0 + issued;
         if (!mbar_wait(&empty[st], ((issued / C::STAGES) & 1) ^ 1, status, INL_DEV_TIMEOUT_PRODUCER)) break;
         mbar_expect_tx(&full[st], C::STAGE_BYTES);
         tma_load_2d(sA + st * C::A_BYTES, &tmA, &full[st], kb * kBK, m0);
@@ -217,78 +215,55 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     if (lane == 0) {
       constexpr uint32_t idesc = umma_idesc_bf16(kBM, BN);
-      bool ok = true;
-      for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
-        const int st = i % C::STAGES;
-        if (!(ok = mbar_wait(&full[st], (i / C::STAGES) & 1, status, INL_DEV_TIMEOUT_MMA))) break;
+      for (int i = 0; i < nkb; ++i) {
+        const int st = i % C::STAGES, chunk = i / C::CHUNK, acc = chunk & 1;
+        if (i % C::CHUNK == 0 && !mbar_wait(&tempty[acc], ((chunk >> 1) & 1) ^ 1, status, INL_DEV_TIMEOUT_MMA)) break;
+        if (!mbar_wait(&full[st], (i / C::STAGES) & 1, status, INL_DEV_TIMEOUT_MMA)) break;
         tc_fence_after();
         const uint64_t a = sw128_kmajor_desc(smem_u32(sA + st * C::A_BYTES));
         const uint64_t b = sw128_kmajor_desc(smem_u32(sB + st * C::B_BYTES));
 #pragma unroll
         for (int kk = 0; kk < kBK / 16; ++kk)
-          umma_bf16(tmem, a + static_cast<uint64_t>(kk * 2), b + static_cast<uint64_t>(kk * 2), idesc,
-                    (i != 0 || kk != 0) ? 1u : 0u);
+          umma_bf16(tmem + acc * BN, a + static_cast<uint64_t>(kk * 2), b + static_cast<uint64_t>(kk * 2), idesc,
+                    (i % C::CHUNK != 0 || kk != 0) ? 1u : 0u);
         umma_commit(&empty[st]);
+        if (i % C::CHUNK == C::CHUNK - 1 || i == nkb - 1) umma_commit(&tfull[acc]);
       }
-      if (ok) umma_commit(tfull);
     }
   } else {
-    // thread = tile row; 16-byte piece j of a 32-column group at j ^ (row & 7)
-    const int quad = warp & 3, half = (warp - 2) >> 2;
-    if (mbar_wait_warp(tfull, 0, status, INL_DEV_TIMEOUT_EPILOGUE)) {
-      tc_fence_after();
-      const int row = quad * 32 + lane;
-      if (m0 + quad * 32 < g.M) {  // warp-uniform
-#pragma unroll 1
-        for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
-          uint32_t v[32];
-          tmem_ld32(tmem + (static_cast<uint32_t>(quad * 32) << 16) + c, v);
-          tmem_ld_wait();
-          uint8_t* dst = part + row * (BN * 4) + c * 4;
+    // thread = tile row (lane quadrant warp % 4), 32 columns. The tensor core's
+    // accumulator truncates (1e-6 of the sum, toward zero, by K = 1024): every
+    // CHUNK blocks it is moved out and summed here, rounded to nearest.
+    const int quad = warp & 3, half = (warp - 2) >> 2, row = quad * 32 + lane;
+    float sum[32];
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint4*>(dst + ((j ^ (row & 7)) << 4)) =
-                make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-        }
-      }
+    for (int j = 0; j < 32; ++j) sum[j] = 0.f;
+    const int chunks = (nkb + C::CHUNK - 1) / C::CHUNK;
+    for (int c = 0; c < chunks; ++c) {
+      const int acc = c & 1;
+      if (!mbar_wait_warp(&tfull[acc], (c >> 1) & 1, status, INL_DEV_TIMEOUT_EPILOGUE)) break;
+      tc_fence_after();
+      uint32_t v[32];
+      tmem_ld32(tmem + (static_cast<uint32_t>(quad * 32) << 16) + acc * BN + half * 32, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) sum[j] += __uint_as_float(v[j]);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty[acc]);
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      *reinterpret_cast<float4*>(cluster_piece<BN>(part, row, half * 8 + j)) =
+          make_float4(sum[4 * j], sum[4 * j + 1], sum[4 * j + 2], sum[4 * j + 3]);
   }
   tc_fence_before();
   cluster_sync_all();  // every partial tile is written
-  // A thread keeps one 4-column piece; the cluster's CTAs take its rows in turn,
-  // four rows (4 S loads) in flight at a time.
-  constexpr int Q = BN / 4, STEP = 256 / Q;
-  if (warp >= 2) {
-    const int tid = threadIdx.x - 64, q = tid % Q, n = n0 + 4 * q;
-    const int rows = min(kBM, g.M - m0);
-    if (n < g.N) {
-      float bias[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) bias[i] = g.bias && n + i < g.N ? __ldg(g.bias + n + i) : 0.f;
-      const uint32_t col = smem_u32(part) + (q >> 3) * 128;
-      for (int r0 = rank * STEP + tid / Q; r0 < rows; r0 += 4 * S * STEP) {
-        float4 v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = make_float4(bias[0], bias[1], bias[2], bias[3]);
-        for (int s = 0; s < S; ++s) {
-          const uint32_t base = mapa_shared(col, s);
-          float4 p[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = min(r0 + i * S * STEP, rows - 1);
-            p[i] = ld_cluster_f4(base + row * (BN * 4) + (((q & 7) ^ (row & 7)) << 4));
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[i].x += p[i].x, v[i].y += p[i].y, v[i].z += p[i].z, v[i].w += p[i].w;
-        }
-        linear_finish_rows<TO, 4>(g, v, m0 + r0, S * STEP, min(4, (rows - r0 + S * STEP - 1) / (S * STEP)), n, wide);
-      }
-    }
-  }
+  if (warp >= 2) cluster_finish<TO, kBN, false>(g, part, threadIdx.x - 64, rank, S, m0, n0, wide != 0);
   cluster_sync_all();  // no CTA leaves while another may still read its partial tile
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, BN);
+    tmem_dealloc(tmem, 2 * BN);
   }
 }
 
@@ -300,20 +275,8 @@ cudaError_t launch_cluster(const CUtensorMap& ta, const CUtensorMap& tb, const L
   static std::atomic<unsigned long long> attr_set{0};
   cudaError_t err = set_smem_limit_once(kern, C::SMEM_BYTES, attr_set);
   if (err != cudaSuccess) return err;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(((g.M + kBM - 1) / kBM) * ((g.N + kBN - 1) / kBN) * S);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = C::SMEM_BYTES;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = S;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kern, ta, tb, g, S, wide, status);
+  const unsigned grid = ((g.M + kBM - 1) / kBM) * ((g.N + kBN - 1) / kBN) * S;
+  return launch_cluster_pdl(kern, grid, kThreads, C::SMEM_BYTES, S, s, ta, tb, g, S, wide, status);
 }
 
 }  // namespace
@@ -328,12 +291,7 @@ cudaError_t linear_cluster(const LinearArgs& g, bool out_bf16, int S, int* statu
   if (!make_tma_2d_bf16(&ta, g.x, g.M, g.K, g.M == 1 ? pad8(g.K) : g.ldx, kBM, kBK) ||
       !make_tma_2d_bf16(&tb, g.w, g.N, g.K, g.N == 1 ? pad8(g.K) : g.ldw, kBN, kBK))
     return cudaErrorInvalidValue;
-  // 4 columns in one access: rows of out and resid on its boundary
-  const int bytes = out_bf16 ? 8 : 16;
-  auto ok = [&](const void* p, long long ld) {
-    return (reinterpret_cast<uintptr_t>(p) % bytes) == 0 && (g.M == 1 || ld % 4 == 0);
-  };
-  const int wide = ok(g.out, g.ldo) && (!g.resid || ok(g.resid, g.ldr));
+  const int wide = linear_wide(g, out_bf16);
   return out_bf16 ? launch_cluster<__nv_bfloat16>(ta, tb, g, S, wide, status, s)
                   : launch_cluster<float>(ta, tb, g, S, wide, status, s);
 }
