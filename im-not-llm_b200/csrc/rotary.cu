@@ -9,8 +9,10 @@
 // before it becomes 32 bits: at position 10^6 a 32-bit product would be off by
 // up to 0.03 radians, the reduced one is off by 3e-8.
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <string>
+#include <type_traits>
 #include <vector>
 
 #include "../../include/inl_cuda.h"
@@ -54,17 +56,35 @@ __device__ __forceinline__ void store_f(T* p, float v) {
   else *p = v;
 }
 
-// cos and sin of pos * inv_freq.
-__device__ __forceinline__ void turn_of(int pos, double inv_freq, float& c, float& s) {
-  const double quarter = static_cast<double>(pos) * inv_freq * 0.63661977236758134308;  // 2 / pi
-  const double q = rint(quarter);
-  const float r = static_cast<float>(quarter - q) * 0.5f;  // half turns, |r| <= 1/4
-  float cr, sr;
-  sincospif(r, &sr, &cr);
-  const int k = static_cast<int>(static_cast<long long>(q)) & 3;
-  const float a = (k & 1) ? sr : cr, b = (k & 1) ? cr : sr;
-  c = (k == 1 || k == 2) ? -a : a;
-  s = (k & 2) ? -b : b;
+// inv_freq (radians per position) as a fraction of a turn per position in
+// 2^-64 turns: pos times it, modulo 2^64, is where the angle ends in its turn,
+// exactly, for any 32-bit position, by one integer product.
+__device__ __forceinline__ uint64_t turn_step(double inv_freq) {
+  const double turns = inv_freq * 0.15915494309189533577;  // 1 / (2 pi)
+  return static_cast<uint64_t>((turns - floor(turns)) * 18446744073709551616.0);
+}
+
+// cos and sin of the angle pos * step: the quarter turn nearest to it by
+// integer arithmetic, and the rest, at most an eighth of a turn, by the Taylor
+// polynomials (the first terms left out are below 2e-9).
+__device__ __forceinline__ void turn_of(int pos, uint64_t step, float& c, float& s) {
+  const int t = static_cast<int>((static_cast<uint64_t>(static_cast<long long>(pos)) * step) >> 32);
+  const int k = (t + (1 << 29)) >> 30;  // wraps to the same quarter at half a turn
+  const float x = static_cast<float>(static_cast<int>(static_cast<unsigned>(t) - (static_cast<unsigned>(k) << 30))) *
+                  1.4629180792671596e-9f;  // 2 pi / 2^32
+  const float x2 = x * x;
+  float cr = fmaf(x2, -1.f / 3628800.f, 1.f / 40320.f);
+  cr = fmaf(x2, cr, -1.f / 720.f);
+  cr = fmaf(x2, cr, 1.f / 24.f);
+  cr = fmaf(x2, cr, -0.5f);
+  cr = fmaf(x2, cr, 1.f);
+  float sr = fmaf(x2, 1.f / 362880.f, -1.f / 5040.f);
+  sr = fmaf(x2, sr, 1.f / 120.f);
+  sr = fmaf(x2, sr, -1.f / 6.f);
+  sr = fmaf(x2 * x, sr, x);
+  const float p = (k & 1) ? sr : cr, q = (k & 1) ? cr : sr;
+  c = ((k + 1) & 2) ? -p : p;
+  s = (k & 2) ? -q : q;
 }
 
 // Any head width, stride and alignment: a warp per (token, head), a lane per
@@ -114,7 +134,7 @@ __global__ void __launch_bounds__(256) rotary_any_kernel(RotaryArgs a) {
     for (int i = lane; i < half; i += 32) {
       const int ja = a.interleaved ? 2 * i : i, jb = a.interleaved ? 2 * i + 1 : i + half;
       float c, s;
-      turn_of(pos, a.inv_freq[i], c, s);
+      turn_of(pos, turn_step(a.inv_freq[i]), c, s);
       c *= a.scale;
       s *= a.scale * a.sin_sign;
       const float va = value(ja), vb = value(jb);
@@ -133,12 +153,264 @@ cudaError_t launch_any(const RotaryArgs& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
+// E consecutive values in one access.
+template <typename T, int E>
+struct Vec {
+  static constexpr int BYTES = E * static_cast<int>(sizeof(T));
+  using Raw = std::conditional_t<BYTES == 16, uint4, std::conditional_t<BYTES == 8, uint2, uint32_t>>;
+  static __device__ __forceinline__ void unpack(const Raw& r, float* v) {
+    const uint32_t* u = reinterpret_cast<const uint32_t*>(&r);
+#pragma unroll
+    for (int i = 0; i < BYTES / 4; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        const float2 f = unpack_bf16x2(u[i]);
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+      } else {
+        v[i] = __uint_as_float(u[i]);
+      }
+    }
+  }
+  static __device__ __forceinline__ Raw pack(const float* v) {
+    Raw r;
+    uint32_t* u = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+    for (int i = 0; i < BYTES / 4; ++i) {
+      if constexpr (sizeof(T) == 2) u[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+      else u[i] = __float_as_uint(v[i]);
+    }
+    return r;
+  }
+};
+
+// The bandwidth-bound form. A head is cut into units of two E-vectors: E pairs
+// of the rotation (vectors i E and half + i E of the half layout, 2 E
+// consecutive features of the interleaved one) or 2 E features that are
+// copied, one unit to a lane, 2^log_lanes lanes to a head. So a lane turns its
+// own registers, without an exchange, and in place writes what it read. A warp
+// takes 2^log_tokens tokens at a time (one, where the heads are many), gives
+// each as many lane groups, and a group takes every step-th head of its token,
+// or of its run of heads (blockIdx.y: some, where the tokens are few). The
+// warp computes its tokens' cos and sin once, into shared memory of its own, so
+// no warp waits for another. A lane asks for a head of the next batch (of KI
+// heads, or of the next tokens) as soon as it has taken this one out of the
+// registers.
+//
+// Bound by memory: 65536 tokens of 24 bf16 heads of 128, rotated 124 us = 6.5
+// TB/s (all of a copy's rate), normed and rotated 145 us = 5.6 TB/s; 20011 f32
+// tokens of 12 heads of 64, interleaved, 25 us = 5.0 TB/s. Tried on the first
+// of these (us): a block per 4 tokens, a barrier between its cos / sin and its
+// heads 175; blocks that walk over tiles, with that barrier 153 to 178; 2 / 4
+// heads in flight 137 / 187 (registers); 8-byte vectors 202; more resident
+// warps at fewer registers 149 and more.
+template <typename T, int E, int NORM, bool INTER, int KI>
+__global__ void __launch_bounds__(256, 2) rotary_vec_kernel(RotaryArgs a, int log_lanes, int log_tokens, int run) {
+  using V = Vec<T, E>;
+  using Raw = typename V::Raw;
+  constexpr int Q = E / 2;          // float4s of a unit's cos and sin, or of its weights
+  extern __shared__ float4 smem4[];  // per warp [tokens][Q][pair units] (cos, sin, cos, sin); [q, k][w, b][Q][units]; steps
+  const int half = a.rot / 2, heads = a.set[0].heads + a.set[1].heads, hq = a.set[0].heads;
+  const int warp = threadIdx.x >> 5, wl = threadIdx.x & 31;
+  const int lane = wl & ((1 << log_lanes) - 1), group = wl >> log_lanes;
+  const int log_step = 5 - log_lanes - log_tokens, step = 1 << log_step;
+  const int pair_units = half / E, units = a.d / (2 * E);
+  const bool active = lane < units, turned = lane < pair_units;
+  auto first_of = [&](int u) { return u >= pair_units ? a.rot + 2 * E * (u - pair_units) : INTER ? 2 * E * u : E * u; };
+  const int f = active ? first_of(lane) : 0;
+  const int gap = turned && !INTER ? half : E;  // from a lane's first vector to its second
+  const int tok = group >> log_step;
+  const int run0 = blockIdx.y * run, run1 = min(run0 + run, heads);  // this block's heads
+  const int h0 = run0 + (group & (step - 1));
+  const int tiles = (a.T - 1) / (1 << log_tokens) + 1;  // of 2^log_tokens tokens
+  const int cs_n = half / 2 << log_tokens;              // float4s of a warp's cos and sin
+  float4* const cs = smem4 + warp * cs_n;
+  float4* const wsm = smem4 + 8 * cs_n;
+  uint64_t* const steps = reinterpret_cast<uint64_t*>(wsm + (NORM == kNoNorm ? 0 : a.d));  // [half]
+
+  auto load = [&](int tile, int h, Raw (&raw)[2]) {
+    const long long row = min((tile << log_tokens) + tok, a.T - 1);
+    h = min(h, run1 - 1);
+    const bool second = h >= hq;
+    const HeadSet& st = a.set[second];
+    const T* x = static_cast<const T*>(st.x) + row * st.ldx + static_cast<int>(second ? h - hq : h) * static_cast<int>(st.hsx) + f;
+    raw[0] = *reinterpret_cast<const Raw*>(x);
+    raw[1] = *reinterpret_cast<const Raw*>(x + gap);
+  };
+  const int turns = half << log_tokens;
+  // lane t: the position of the warp's token t
+  auto load_pos = [&](int tile) {
+    return half && wl < 1 << log_tokens ? a.pos[min((tile << log_tokens) + wl, a.T - 1)] : 0;
+  };
+
+  int tile = blockIdx.x * 8 + warp;
+  const int tile_step = gridDim.x * 8;
+  Raw raw[KI][2];
+  int pos = 0;
+  if (tile < tiles) {
+#pragma unroll
+    for (int k = 0; k < KI; ++k) load(tile, h0 + k * step, raw[k]);
+    pos = load_pos(tile);
+  }
+  for (int i = threadIdx.x; i < half; i += 256) steps[i] = turn_step(a.inv_freq[i]);
+  if constexpr (NORM != kNoNorm) {
+    float* const wf = reinterpret_cast<float*>(wsm);
+    for (int i = threadIdx.x; i < 2 * units * 2 * E; i += 256) {
+      const int k = i / (units * 2 * E), u = i / (2 * E) % units, e = i % (2 * E);
+      const int ff = first_of(u) + (e < E ? e : (u < pair_units && !INTER ? half : E) + e - E);
+      const HeadSet& st = a.set[k];
+      float* to = wf + ((2 * k * Q + e / 4) * units + u) * 4 + e % 4;
+      *to = st.w ? st.w[ff] : 1.f;
+      if constexpr (NORM == kLayer) to[4 * Q * units] = st.b ? st.b[ff] : 0.f;
+    }
+  }
+  __syncthreads();
+
+  for (; tile < tiles; tile += tile_step) {
+    const int next = tile + tile_step;
+    __syncwarp();  // the last tokens' cos and sin have been read
+#pragma unroll 2
+    for (int i = wl; i < (turns + 31 & ~31); i += 32) {  // whole warps: the shuffle
+      const int t = log_tokens ? min(i / half, (1 << log_tokens) - 1) : 0, p = i - t * half;
+      const int at = __shfl_sync(0xffffffffu, pos, t);
+      if (i < turns) {
+        float co, si;
+        turn_of(at, steps[p], co, si);
+        reinterpret_cast<float2*>(cs)[t * half + (p % E / 2 * pair_units + p / E) * 2 + (p & 1)] =
+            make_float2(co * a.scale, si * (a.scale * a.sin_sign));
+      }
+    }
+    if (next < tiles) pos = load_pos(next);
+    __syncwarp();
+    float c[E], sn[E];
+    if (turned) {
+#pragma unroll
+      for (int j = 0; j < Q; ++j) {
+        const float4 r = cs[(tok * Q + j) * pair_units + lane];
+        c[2 * j] = r.x, sn[2 * j] = r.y, c[2 * j + 1] = r.z, sn[2 * j + 1] = r.w;
+      }
+    }
+    const long long row = (tile << log_tokens) + tok;
+    const bool mine = active && row < a.T;
+    for (int b = 0; run0 + b < run1; b += KI * step) {
+      const bool more = run0 + b + KI * step < run1;  // heads of this token after the batch
+#pragma unroll
+      for (int k = 0; k < KI; ++k) {
+        const int h = h0 + b + k * step;
+        const bool second = h >= hq;
+        float v[2 * E];
+        V::unpack(raw[k][0], v);
+        V::unpack(raw[k][1], v + E);
+        if (more || next < tiles) load(more ? tile : next, more ? h + KI * step : h0 + k * step, raw[k]);
+        if (run0 + b + k * step >= run1) continue;  // the same for the whole warp
+        if constexpr (NORM != kNoNorm) {
+          const float rd = 1.f / static_cast<float>(a.d);
+          if constexpr (NORM == kLayer) {
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 2 * E; ++e) sum += v[e];
+            if (!active) sum = 0.f;
+            for (int o = 1 << log_lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const float mean = sum * rd;
+#pragma unroll
+            for (int e = 0; e < 2 * E; ++e) v[e] -= mean;
+          }
+          float ss = 0.f;
+#pragma unroll
+          for (int e = 0; e < 2 * E; ++e) ss = fmaf(v[e], v[e], ss);
+          if (!active) ss = 0.f;
+          for (int o = 1 << log_lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          const float inv = rsqrtf(fmaf(ss, rd, a.eps));
+          const float4* w = wsm + (second ? 2 * Q * units : 0) + (active ? lane : 0);
+#pragma unroll
+          for (int j = 0; j < Q; ++j) {
+            const float4 q = w[j * units];
+            v[4 * j] *= inv * q.x, v[4 * j + 1] *= inv * q.y, v[4 * j + 2] *= inv * q.z, v[4 * j + 3] *= inv * q.w;
+            if constexpr (NORM == kLayer) {
+              const float4 r = w[(Q + j) * units];
+              v[4 * j] += r.x, v[4 * j + 1] += r.y, v[4 * j + 2] += r.z, v[4 * j + 3] += r.w;
+            }
+          }
+        }
+        if (turned) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const int ia = INTER ? 2 * e : e, ib = INTER ? 2 * e + 1 : E + e;
+            const float x = v[ia], y = v[ib];
+            v[ia] = x * c[e] - y * sn[e];
+            v[ib] = y * c[e] + x * sn[e];
+          }
+        }
+        if (mine && h < run1) {
+          const HeadSet& st = a.set[second];
+          T* out = static_cast<T*>(st.out) + row * st.ldo + static_cast<int>(second ? h - hq : h) * a.d + f;
+          *reinterpret_cast<Raw*>(out) = V::pack(v);
+          *reinterpret_cast<Raw*>(out + gap) = V::pack(v + E);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int E, int NORM, bool INTER>
+cudaError_t launch_vec(const RotaryArgs& a, cudaStream_t s) {
+  constexpr int KI = 3;
+  const int units = a.d / (2 * E), heads = a.set[0].heads + a.set[1].heads, half = a.rot / 2;
+  int log_lanes = 0;
+  while (1 << log_lanes < units) ++log_lanes;
+  const int groups = 32 >> log_lanes, sms = num_sms_cached();
+  // several tokens to a warp where one token's heads would leave groups or the KI
+  // loads of a lane idle, as long as the SMs keep 8 warps each
+  int log_tokens = 0;
+  while (2 << log_tokens <= groups && (2ll << log_tokens) * heads <= static_cast<long long>(KI) * groups &&
+         half << log_tokens <= 128 && a.T >> (log_tokens + 1) >= 8 * sms)
+    ++log_tokens;
+  // and a token's heads in several runs where the tokens are fewer than that
+  const int batch = KI * (groups >> log_tokens);
+  int runs = 1;
+  while (runs < 64 && static_cast<long long>(a.T) * runs < 8 * sms && heads > batch * runs) ++runs;
+  const int run = ((heads + runs - 1) / runs + batch - 1) / batch * batch;
+  runs = (heads + run - 1) / run;
+  const int tiles = (a.T - 1) / (1 << log_tokens) + 1;
+  const size_t smem = (static_cast<size_t>(half) << log_tokens) * 64 + (NORM == kNoNorm ? 0 : 16 * a.d) + 8 * half;
+  auto kern = rotary_vec_kernel<T, E, NORM, INTER, KI>;
+  const dim3 grid(std::min((tiles - 1) / 8 + 1, sms * 4), runs);
+  kern<<<grid, 256, smem, s>>>(a, log_lanes, log_tokens, run);
+  return cudaGetLastError();
+}
+
+// Whether heads, pairs and rows come apart into E-vectors, 32 units to a head at most.
+bool vec_takes(const RotaryArgs& a, int E, int elem) {
+  if (a.rot % (2 * E) || a.d % (2 * E) || a.d > 64 * E) return false;
+  for (const HeadSet& h : a.set) {
+    if (h.heads == 0) continue;
+    if ((reinterpret_cast<uintptr_t>(h.x) | reinterpret_cast<uintptr_t>(h.out)) % static_cast<unsigned>(E * elem))
+      return false;
+    if (a.T > 1 && (h.ldx % E || h.ldo % E)) return false;
+    if (h.heads > 1 && (h.hsx % E || h.hsx * h.heads > INT_MAX)) return false;  // 32-bit offsets inside a row
+    if (static_cast<long long>(h.heads) * a.d > INT_MAX) return false;
+  }
+  return true;
+}
+
+template <typename T, int NORM>
+cudaError_t launch_norm(const RotaryArgs& a, cudaStream_t s) {
+  constexpr int kMost = 16 / static_cast<int>(sizeof(T));
+  auto with = [&](auto e) {
+    constexpr int E = decltype(e)::value;
+    return a.interleaved ? launch_vec<T, E, NORM, true>(a, s) : launch_vec<T, E, NORM, false>(a, s);
+  };
+  if (vec_takes(a, kMost, sizeof(T))) return with(std::integral_constant<int, kMost>());
+  if (vec_takes(a, kMost / 2, sizeof(T))) return with(std::integral_constant<int, kMost / 2>());
+  if constexpr (sizeof(T) == 2)
+    if (vec_takes(a, 2, sizeof(T))) return with(std::integral_constant<int, 2>());
+  return launch_any<T, NORM>(a, s);
+}
+
 template <typename T>
 cudaError_t launch_rotary(const RotaryArgs& a, int norm, cudaStream_t s) {
   switch (norm) {
-    case kNoNorm: return launch_any<T, kNoNorm>(a, s);
-    case kRms: return launch_any<T, kRms>(a, s);
-    default: return launch_any<T, kLayer>(a, s);
+    case kNoNorm: return launch_norm<T, kNoNorm>(a, s);
+    case kRms: return launch_norm<T, kRms>(a, s);
+    default: return launch_norm<T, kLayer>(a, s);
   }
 }
 
@@ -149,7 +421,7 @@ int bad(const char* what, const char* why) {
 // Checks that need no device. Row widths as 64-bit products.
 int check_rotary(const char* what, int dtype, int T, int d, int rot, const RotaryArgs& a) {
   if (dtype != INL_DTYPE_F32 && dtype != INL_DTYPE_BF16) return bad(what, "dtype is f32 or bf16");
-  if (T < 0 || d <= 0) return bad(what, "T >= 0 and d > 0");
+  if (T < 0 || T > 1 << 30 || d <= 0) return bad(what, "T from 0 to 2^30, d > 0");
   if (rot < 0 || rot > d || (rot & 1)) return bad(what, "rotary_dim is even and at most d");
   if (!std::isfinite(a.scale)) return bad(what, "scale is finite");
   for (const HeadSet& h : a.set) {
