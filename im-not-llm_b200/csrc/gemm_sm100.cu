@@ -34,6 +34,7 @@ constexpr int kBM = 128;
 constexpr int kBK = 64;  // one 128-byte swizzle row of bf16
 constexpr int kEpiWarps = 8;  // two warps per TMEM lane quadrant, each owning half of the tile's columns
 constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kLongBlocks = 8;  // K blocks between promotions of INL_EPI_LINEAR_F32_LONG
 
 template <int BN>
 struct GemmCfg {
@@ -230,6 +231,45 @@ __device__ __forceinline__ void turn_store32(uint8_t* buf, const float (&v)[32],
   }
 }
 
+// Bias of 32 columns, zero where there is none.
+__device__ __forceinline__ void linear_bias32(float (&v)[32], const EpiArgs& e, int col) {
+  const int left = e.N - col;
+  if (e.bias == nullptr) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = 0.f;
+  } else if (e.aligned && left >= 32) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float4 b = __ldg(reinterpret_cast<const float4*>(e.bias + col) + j);
+      v[4 * j] = b.x, v[4 * j + 1] = b.y, v[4 * j + 2] = b.z, v[4 * j + 3] = b.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = j < left ? __ldg(e.bias + col + j) : 0.f;
+  }
+}
+
+// Activation, residual and store of 32 columns of this thread's row (bias included in v).
+template <bool F32>
+__device__ __forceinline__ void linear_store32(float (&v)[32], const EpiArgs& e, OutStage& st, int row, int col,
+                                               int lane) {
+  const int row0 = row - lane;
+  linear_act<std::conditional_t<F32, float, __nv_bfloat16>>(v, e.act);
+  if constexpr (F32) {
+    turn_store32(st.buf, v, e, static_cast<float*>(e.out), reinterpret_cast<const float*>(e.resid), row0, col, lane);
+  } else if (e.aligned) {
+    if (e.resid != nullptr && row < e.M) {
+      float rr[32];
+      load_row32_bf16(e.resid + static_cast<long long>(row) * e.ldr + col, rr, e.N - col);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] += rr[j];
+    }
+    stage_store32(st, v, col, row0, lane);
+  } else {
+    turn_store32(st.buf, v, e, static_cast<__nv_bfloat16*>(e.out), e.resid, row0, col, lane);
+  }
+}
+
 // One q or k head of width D in TMEM columns [c0, c0 + D) of this thread's row:
 // RMSNorm with weight w, then half-split RoPE at position p, stored through st
 // at output columns col0 .. col0 + D of rows row0 .. row0 + 31.
@@ -403,40 +443,13 @@ __device__ __forceinline__ void epilogue_tile(uint32_t t_row, int row, int n0, i
 #pragma unroll 1
     for (int c = 0; c < HW; c += 32) {
       const int col = n0 + half * HW + c;
-      const int left = e.N - col;
-      if (left <= 0) break;  // warp-uniform
+      if (col >= e.N) break;  // warp-uniform
       tmem_ld32(t_row + half * HW + c, r);
-      if (e.bias == nullptr) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = 0.f;
-      } else if (e.aligned && left >= 32) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float4 b = __ldg(reinterpret_cast<const float4*>(e.bias + col) + j);
-          v[4 * j] = b.x, v[4 * j + 1] = b.y, v[4 * j + 2] = b.z, v[4 * j + 3] = b.w;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = j < left ? __ldg(e.bias + col + j) : 0.f;
-      }
+      linear_bias32(v, e, col);
       tmem_ld_wait();
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(r[j]);
-      linear_act<std::conditional_t<EPI == INL_EPI_LINEAR_F32, float, __nv_bfloat16>>(v, e.act);
-      if constexpr (EPI == INL_EPI_LINEAR_F32) {
-        turn_store32(st.buf, v, e, static_cast<float*>(e.out), reinterpret_cast<const float*>(e.resid), row0, col,
-                     lane);
-      } else if (e.aligned) {
-        if (e.resid != nullptr && row_ok) {
-          float rr[32];
-          load_row32_bf16(e.resid + static_cast<long long>(row) * e.ldr + col, rr, left);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] += rr[j];
-        }
-        stage_store32(st, v, col, row0, lane);
-      } else {
-        turn_store32(st.buf, v, e, static_cast<__nv_bfloat16*>(e.out), e.resid, row0, col, lane);
-      }
+      linear_store32<EPI == INL_EPI_LINEAR_F32>(v, e, st, row, col, lane);
     }
   } else {
 #pragma unroll 1
@@ -525,6 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int k_blocks = (K + kBK - 1) / kBK;
   const int splits = e.splits > 1 ? e.splits : 1;
   const int num_units = num_tiles * splits;
+  constexpr bool LONG = EPI == INL_EPI_LINEAR_F32_LONG;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -593,36 +607,44 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       for (int u = blockIdx.x; u < num_units && ok; u += gridDim.x) {
         const Unit w = unit_of(u, splits, k_blocks);
-        if (!mbar_wait(&tempty[acc], acc_phase ^ 1, status, INL_DEV_TIMEOUT_MMA)) break;
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
-        for (int kb = w.kb0; kb < w.kb1; ++kb) {
-          if (!mbar_wait(&full[stage], phase, status, INL_DEV_TIMEOUT_MMA)) {
+        int kb_first = w.kb0;
+        do {
+          const int kb_end = LONG ? min(w.kb1, kb_first + kLongBlocks) : w.kb1;
+          if (!mbar_wait(&tempty[acc], acc_phase ^ 1, status, INL_DEV_TIMEOUT_MMA)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          // Descriptors differ from the ring's base descriptors only in the
-          // start-address field (address >> 4, 14 bits; shared memory < 256 KB).
-          const uint64_t a_desc = a_desc0 + static_cast<uint64_t>((stage * C::A_BYTES) >> 4);
-          const uint64_t b_desc = b_desc0 + static_cast<uint64_t>((stage * C::B_BYTES) >> 4);
+          const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
+          for (int kb = kb_first; kb < kb_end; ++kb) {
+            if (!mbar_wait(&full[stage], phase, status, INL_DEV_TIMEOUT_MMA)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            // Descriptors differ from the ring's base descriptors only in the
+            // start-address field (address >> 4, 14 bits; shared memory < 256 KB).
+            const uint64_t a_desc = a_desc0 + static_cast<uint64_t>((stage * C::A_BYTES) >> 4);
+            const uint64_t b_desc = b_desc0 + static_cast<uint64_t>((stage * C::B_BYTES) >> 4);
 #pragma unroll
-          for (int kk = 0; kk < kBK / 16; ++kk) {
-            umma_bf16(d_tmem, a_desc + static_cast<uint64_t>(kk * 2), b_desc + static_cast<uint64_t>(kk * 2), idesc,
-                      (kb != w.kb0 || kk != 0) ? 1u : 0u);
+            for (int kk = 0; kk < kBK / 16; ++kk) {
+              umma_bf16(d_tmem, a_desc + static_cast<uint64_t>(kk * 2), b_desc + static_cast<uint64_t>(kk * 2), idesc,
+                        (kb != kb_first || kk != 0) ? 1u : 0u);
+            }
+            umma_commit(&empty[stage]);
+            if (++stage == C::STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
           }
-          umma_commit(&empty[stage]);
-          if (++stage == C::STAGES) {
-            stage = 0;
-            phase ^= 1;
+          if (!ok) break;
+          umma_commit(&tfull[acc]);
+          if (++acc == 2) {
+            acc = 0;
+            acc_phase ^= 1;
           }
-        }
-        if (!ok) break;
-        umma_commit(&tfull[acc]);
-        if (++acc == 2) {
-          acc = 0;
-          acc_phase ^= 1;
-        }
+          kb_first = kb_end;
+        } while (LONG && kb_first < w.kb1);
       }
     }
   } else {
@@ -635,6 +657,47 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int u = blockIdx.x; u < num_units; u += gridDim.x) {
       const Unit w = unit_of(u, splits, k_blocks);
       const int mb = w.tile / n_tiles, nb = w.tile - (w.tile / n_tiles) * n_tiles;
+      if constexpr (LONG) {
+        // this warp's half of the tile, summed in registers over the parts of K
+        constexpr int HW = BN / 2;
+        float sum[HW];
+#pragma unroll
+        for (int j = 0; j < HW; ++j) sum[j] = 0.f;
+        bool ok = true;
+        for (int kb = w.kb0; kb < w.kb1; kb += kLongBlocks) {
+          if (!(ok = mbar_wait_warp(&tfull[acc], acc_phase, status, INL_DEV_TIMEOUT_EPILOGUE))) break;
+          tc_fence_after();
+          const uint32_t t = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
+                             static_cast<uint32_t>(acc * BN + half * HW);
+#pragma unroll
+          for (int c = 0; c < HW; c += 32) {
+            uint32_t r[32];
+            tmem_ld32(t + c, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sum[c + j] += __uint_as_float(r[j]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&tempty[acc]);
+          if (++acc == 2) {
+            acc = 0;
+            acc_phase ^= 1;
+          }
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < HW; c += 32) {
+          const int col = nb * BN + half * HW + c;
+          if (col >= N) break;  // warp-uniform
+          float v[32];
+          linear_bias32(v, e, col);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += sum[c + j];
+          linear_store32<true>(v, e, st, mb * kBM + quad * 32 + lane, col, lane);
+        }
+        continue;
+      }
       if (!mbar_wait_warp(&tfull[acc], acc_phase, status, INL_DEV_TIMEOUT_EPILOGUE)) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * BN);
@@ -948,11 +1011,10 @@ cudaError_t dispatch_act(int act, const CUtensorMap& ta, const CUtensorMap& tb, 
 template <int EPI>
 cudaError_t launch_linear(int bn, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& to, int M, int N,
                           int K, const EpiArgs& e, int* status, cudaStream_t s) {
-  switch (bn) {
-    case 256: return launch_gemm_pair<EPI, 0>(ta, tb, to, M, N, K, e, status, 0, s);
-    case 128: return launch_gemm<128, EPI, 0>(ta, tb, to, M, N, K, e, status, 0, s);
-    default: return launch_gemm<64, EPI, 0>(ta, tb, to, M, N, K, e, status, 0, s);
-  }
+  if constexpr (EPI != INL_EPI_LINEAR_F32_LONG)
+    if (bn == 256) return launch_gemm_pair<EPI, 0>(ta, tb, to, M, N, K, e, status, 0, s);
+  return bn == 128 ? launch_gemm<128, EPI, 0>(ta, tb, to, M, N, K, e, status, 0, s)
+                   : launch_gemm<64, EPI, 0>(ta, tb, to, M, N, K, e, status, 0, s);
 }
 
 }  // namespace
@@ -1134,7 +1196,13 @@ int gemm_bf16_linear(const GemmArgs& g, bool out_bf16, cudaStream_t stream) {
     return ((g.M + bm - 1) / bm * ((g.N + bn - 1) / bn) + at_once - 1) / at_once;
   };
   const long long t256 = 8 * waves(256, 256, sms / 2), t128 = 6 * waves(128, 128, sms), t64 = 5 * waves(128, 64, sms);
-  const int bn = t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64;
+  // The tensor core's f32 accumulator truncates: a sum of K = 1024 products is
+  // off by 1e-6 of itself toward zero, one of 4096 by 4.4e-6, which an f32
+  // result shows. Past 512, such a sum is moved out every 512 of K and added in
+  // registers, rounded to nearest (5e-7 at any K; 64 registers a thread, so
+  // tiles of at most 128 columns).
+  const bool parts = !out_bf16 && g.K > kLongBlocks * kBK;
+  const int bn = !parts && t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64;
   CUtensorMap ta, tb, to;
   if (!make_kmajor_map(&ta, g.A, g.M, g.K, lda, kBM)) return -2;
   if (!make_kmajor_map(&tb, g.W, g.N, g.K, ldw, bn == 256 ? 128 : bn)) return -2;
@@ -1144,6 +1212,7 @@ int gemm_bf16_linear(const GemmArgs& g, bool out_bf16, cudaStream_t stream) {
     return -2;
   const cudaError_t err =
       out_bf16 ? launch_linear<INL_EPI_LINEAR_BF16>(bn, ta, tb, to, g.M, g.N, g.K, e, g.status, stream)
+      : parts  ? launch_linear<INL_EPI_LINEAR_F32_LONG>(bn, ta, tb, to, g.M, g.N, g.K, e, g.status, stream)
                : launch_linear<INL_EPI_LINEAR_F32>(bn, ta, tb, to, g.M, g.N, g.K, e, g.status, stream);
   return err == cudaSuccess ? 0 : -3;
 }

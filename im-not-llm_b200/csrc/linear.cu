@@ -1,8 +1,6 @@
-// Linear layer out = act(x w^T + bias) + resid (inl_cuda_linear).
-//
-// linear_any_kernel takes every shape, stride and alignment: 64 x 64 outputs per
-// CTA, 16-deep K slices staged in shared memory as f32, 4 x 4 outputs per
-// thread on FFMA.
+// Linear layer out = act(x w^T + bias) + resid (inl_cuda_linear): the entry
+// point, the choice of the kernel, and linear_rows_kernel, the FFMA form for few
+// rows of f32 operands, or of operands no vector load aligns with.
 #include <algorithm>
 #include <cmath>
 #include <string>
@@ -18,61 +16,93 @@ namespace inl {
 
 namespace {
 
-template <typename TX, typename TO>
-__global__ void __launch_bounds__(256) linear_any_kernel(LinearArgs g) {
-  constexpr int BM = 64, BN = 64, BK = 16;
-  __shared__ float xs[BK][BM + 4];
-  __shared__ float ws[BK][BN + 4];
-  const TX* x = static_cast<const TX*>(g.x);
-  const TX* w = static_cast<const TX*>(g.w);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int n_tiles = (g.N + BN - 1) / BN;
-  const long long tiles = static_cast<long long>((g.M + BM - 1) / BM) * n_tiles;
-  for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const int m0 = static_cast<int>(tile / n_tiles) * BM, n0 = static_cast<int>(tile % n_tiles) * BN;
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < g.K; k0 += BK) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int idx = threadIdx.x + i * 256, r = idx >> 4, kk = idx & 15;
-        const bool k_ok = kk < g.K - k0;
-        xs[kk][r] = (k_ok && r < g.M - m0) ? load_f(x + (m0 + r) * g.ldx + k0 + kk) : 0.f;
-        ws[kk][r] = (k_ok && r < g.N - n0) ? load_f(w + (n0 + r) * g.ldw + k0 + kk) : 0.f;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int kk = 0; kk < BK; ++kk) {
-        const float4 a = *reinterpret_cast<const float4*>(&xs[kk][ty * 4]);
-        const float4 b = *reinterpret_cast<const float4*>(&ws[kk][tx * 4]);
-        const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
-      }
-      __syncthreads();
+// V consecutive values of a row from k on, zero past K. V = 4 wants them on a 16-byte boundary.
+template <typename T, int V>
+__device__ __forceinline__ void load_values(const T* row, int k, int K, float (&v)[V]) {
+  if constexpr (V == 4) {
+    if (K - k >= 4) {
+      const float4 q = __ldg(reinterpret_cast<const float4*>(row + k));
+      v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+      return;
     }
+  }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (ty * 4 + i >= g.M - m0) continue;
-      const long long m = m0 + ty * 4 + i;
+  for (int i = 0; i < V; ++i) v[i] = i < K - k ? load_f(row + k + i) : 0.f;
+}
+
+// A read of w, like linear_skinny_kernel, on FFMA: a CTA owns R rows of w and MT
+// rows of x, its 8 warps take turns of K, a lane V values of each row. f32 sums:
+// over a lane's share of K, then the lanes and the warps in order. One f32 row
+// x 1024 x 1024: 2.6 us; x 4096 x 1024: 6.0 us = 2.8 TB/s; 8 rows of the
+// latter 13.5 us, bound by the loads of x, which every CTA makes again.
+template <typename TX, typename TO, int MT, int R, int V>
+__global__ void __launch_bounds__(256, MT < 8 ? 3 : 2) linear_rows_kernel(LinearArgs g) {
+  __shared__ float red[8][MT * R];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n0 = blockIdx.x * R;
+  const TX* w[R];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (tx * 4 + j >= g.N - n0) continue;
-        const int n = n0 + tx * 4 + j;
-        float v = act_exact(acc[i][j] + (g.bias ? g.bias[n] : 0.f), g.act);
-        if (g.resid) v += load_f(static_cast<const TO*>(g.resid) + m * g.ldr + n);
-        store_f(static_cast<TO*>(g.out) + m * g.ldo + n, v);
+  for (int r = 0; r < R; ++r) w[r] = static_cast<const TX*>(g.w) + min(n0 + r, g.N - 1) * g.ldw;
+  for (int m0 = blockIdx.y * MT; m0 < g.M; m0 += gridDim.y * MT) {
+    const TX* x[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) x[m] = static_cast<const TX*>(g.x) + min(m0 + m, g.M - 1) * g.ldx;
+    float acc[MT][R] = {};
+#pragma unroll(MT < 8 ? 2 : 1)
+    for (int k = (warp * 32 + lane) * V; k < g.K; k += 256 * V) {
+      float wv[R][V], xv[MT][V];
+#pragma unroll
+      for (int r = 0; r < R; ++r) load_values<TX, V>(w[r], k, g.K, wv[r]);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) load_values<TX, V>(x[m], k, g.K, xv[m]);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[m][r] = fmaf(xv[m][i], wv[r][i], acc[m][r]);
+    }
+    __syncthreads();  // the rows before have been summed
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float t = warp_sum(acc[m][r]);
+        if (lane == 0) red[warp][m * R + r] = t;
       }
+    __syncthreads();
+    if (threadIdx.x < MT * R) {
+      const int m = m0 + threadIdx.x / R, n = n0 + threadIdx.x % R;
+      float v = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v += red[i][threadIdx.x];
+      if (m < g.M && n < g.N) linear_finish(g, v, static_cast<long long>(m), n, static_cast<TO*>(g.out));
     }
   }
 }
 
-template <typename TX, typename TO>
-cudaError_t launch_linear_any(const LinearArgs& g, cudaStream_t s) {
-  const long long tiles = static_cast<long long>((g.M + 63) / 64) * ((g.N + 63) / 64);
-  linear_any_kernel<TX, TO><<<static_cast<unsigned>(std::min<long long>(tiles, 1 << 20)), 256, 0, s>>>(g);
+template <typename TX, typename TO, int MT, int V>
+cudaError_t launch_rows(const LinearArgs& g, cudaStream_t s) {
+  constexpr int R = 4;
+  const dim3 grid((g.N + R - 1) / R, std::min((g.M + MT - 1) / MT, 65535));
+  linear_rows_kernel<TX, TO, MT, R, V><<<grid, 256, 0, s>>>(g);
   return cudaGetLastError();
+}
+
+template <typename TX, typename TO, int V>
+cudaError_t launch_rows_for(const LinearArgs& g, cudaStream_t s) {
+  if (g.M == 1) return launch_rows<TX, TO, 1, V>(g, s);
+  if (g.M <= 4) return launch_rows<TX, TO, 4, V>(g, s);
+  return launch_rows<TX, TO, 8, V>(g, s);
+}
+
+cudaError_t linear_rows(const LinearArgs& g, bool x_bf16, bool out_bf16, bool aligned, cudaStream_t s) {
+  if (x_bf16)
+    return out_bf16 ? launch_rows_for<__nv_bfloat16, __nv_bfloat16, 1>(g, s)
+                    : launch_rows_for<__nv_bfloat16, float, 1>(g, s);
+  if (aligned)
+    return out_bf16 ? launch_rows_for<float, __nv_bfloat16, 4>(g, s) : launch_rows_for<float, float, 4>(g, s);
+  return out_bf16 ? launch_rows_for<float, __nv_bfloat16, 1>(g, s) : launch_rows_for<float, float, 1>(g, s);
 }
 
 int bad(const char* why) { return record_error(INL_ERR_INVALID_INPUT, std::string("linear: ") + why); }
@@ -91,14 +121,15 @@ int cluster_size(const LinearArgs& g, int sms) {
   return tiles * 2 <= sms && k_blocks >= 6 ? 2 : 1;
 }
 
-// The same for the f32 kernel, whose CTAs take one tile each: the S of the
-// least (waves over the SMs) x (blocks of 32 k + 4 for a tile's start and end).
-// Measured (us), S = 1 / 2 / 4 / 8: 1024 x 1024 x 1024 36 / 21 / 29 / 74;
+// The same for the kernels whose CTAs take one 128 x 128 tile each (f32, and
+// rows of any alignment): the S of the least (waves over the SMs) x (blocks of
+// 128 bytes of k + 4 for a tile's start and end).
+// Measured (us), f32, S = 1 / 2 / 4 / 8: 1024 x 1024 x 1024 36 / 21 / 29 / 74;
 // 1024 x 4096 x 1024 72 / 85 / 117 / 262; 8192 x 1024 x 4096 478 / 444 / 575 /
 // 906; 4253 x 768 x 768 66 / 58 / 94 / 201; 32 x 1024 x 1024 40 / 22 / 15 / 12.
-int f32_cluster_size(const LinearArgs& g, int sms) {
+int tile_cluster_size(const LinearArgs& g, int bk, int sms) {
   const long long tiles = static_cast<long long>((g.M + 127) / 128) * ((g.N + 127) / 128);
-  const int k_blocks = (g.K + 31) / 32;
+  const int k_blocks = (g.K + bk - 1) / bk;
   int best = 1;
   long long least = -1;
   for (int S = 1; S <= 8 && S <= k_blocks; S *= 2) {
@@ -140,16 +171,20 @@ int linear(const LinearArgs& g, int dtype, int out_dtype, int* status, cudaStrea
   if (xb && gemm_bf16_linear_takes(t)) {
     if (g.M <= 32 || (g.M <= 64 && g.N <= 8 * sms)) return launched("linear", linear_skinny(g, ob, s));
     const int S = cluster_size(g, sms);
-    if (S > 1) return launched("linear", linear_cluster(g, ob, S, status, s));
+    if (S > 1) return launched("linear", linear_cluster(g, ob, true, S, status, s));
     const int rc = gemm_bf16_linear(t, ob, s);
     if (rc == 0) return INL_OK;
     return record_error(INL_ERR_INFERENCE, rc == -3 ? "linear launch failed" : "linear: no TMA map for x, w or out");
   }
-  if (!xb && linear_f32_takes(g)) return launched("linear", linear_f32(g, ob, f32_cluster_size(g, sms), status, s));
-  return launched("linear", xb ? (ob ? launch_linear_any<__nv_bfloat16, __nv_bfloat16>(g, s)
-                                     : launch_linear_any<__nv_bfloat16, float>(g, s))
-                               : (ob ? launch_linear_any<float, __nv_bfloat16>(g, s)
-                                     : launch_linear_any<float, float>(g, s)));
+  const bool aligned = xb ? gemm_bf16_linear_takes(t) : linear_f32_takes(g);
+  // Few rows, where the product is a read of w. Measured (us), linear_rows /
+  // the tensor-core kernel, f32, K = 1024: M = 1, N = 4096 6.0 / 13.5; 8 x 4096
+  // 13.5 / 14.1; 16 x 1024 8.1 / 10.8; 16 x 4096 23 / 14; 32 x 1024 14 / 11.4;
+  // bf16 rows of odd strides: 8 x 1024 5.0 / 10.8; 32 x 1024 15 / 12.
+  if (g.K == 0 || g.M <= 8 || (g.M <= 16 && g.N <= 8 * sms))
+    return launched("linear", linear_rows(g, xb, ob, aligned, s));
+  if (xb) return launched("linear", linear_cluster(g, ob, false, tile_cluster_size(g, 64, sms), status, s));
+  return launched("linear", linear_f32(g, ob, aligned, tile_cluster_size(g, 32, sms), status, s));
 }
 
 }  // namespace

@@ -261,15 +261,109 @@ cudaError_t launch_cluster_pdl(void (*kern)(Params...), unsigned grid, int threa
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
 
-// linear_sm100.cu. Both want 16-byte rows of x and w (gemm_bf16_linear_takes).
-// At most 64 rows.
+// ------------------------------------------------------------------ rows of any alignment
+// Sixteen warps fetch a stage of 256 rows (128 of x, 128 of w) x 128 bytes of K,
+// 16 rows each, a 4-byte word to a lane, into registers, two stages ahead (64 KB
+// in flight per SM).
+constexpr int kLoadWarps = 16, kLoadRows = 256 / kLoadWarps;
+
+// One loading warp's rows. A bf16 row may start in the middle of a word: then
+// the lanes read the words it lies in, and each takes the upper half of its own
+// and the lower half of its neighbour's (the last lane's comes from `extra`,
+// which lane j reads for row j). Only words with an element of the row in them
+// are read; what is past K or past the matrix becomes zero. Blocks that hold
+// none of that go without the checks: it is instructions that bound this.
+template <typename T>
+struct RowWords {
+  static constexpr int E = 4 / static_cast<int>(sizeof(T));
+  uintptr_t row0;  // this lane's first word in row 0
+  long long step;
+  int valid, K, lane;
+  uint32_t shift_even, shift_odd;  // 16 where rows 0, 2, ... (1, 3, ...) start in the middle of a word
+
+  __device__ __forceinline__ RowWords(const void* base, long long ld, int first, int rows, int K_, int lane_)
+      : row0(reinterpret_cast<uintptr_t>(base) + first * ld * static_cast<long long>(sizeof(T)) + 4 * lane_),
+        step(ld * static_cast<long long>(sizeof(T))),
+        valid(min(rows - first, kLoadRows)),
+        K(K_),
+        lane(lane_),
+        shift_even(static_cast<uint32_t>(row0 & 2) * 8),
+        shift_odd(static_cast<uint32_t>((row0 + step) & 2) * 8) {}
+  __device__ __forceinline__ bool inside(int k0) const { return valid == kLoadRows && k0 + 32 * E + 1 < K; }
+  __device__ __forceinline__ uint32_t shift(int j) const { return j & 1 ? shift_odd : shift_even; }
+  static __device__ __forceinline__ uint32_t word(uintptr_t at) {
+    return __ldg(reinterpret_cast<const uint32_t*>(at & ~uintptr_t(3)));
+  }
+  __device__ __forceinline__ void load(uint32_t (&a)[kLoadRows], uint32_t& extra, int k0) const {
+    uintptr_t r = row0 + static_cast<long long>(k0) * static_cast<int>(sizeof(T));
+    // row `lane`, the word after the last lane's
+    const uintptr_t after = r + lane * step + 128 - 4 * lane;
+    if (inside(k0)) {
+      if (E == 2) extra = word(lane < kLoadRows ? after : r);
+#pragma unroll
+      for (int j = 0; j < kLoadRows; ++j, r += step) a[j] = word(r);
+    } else {
+      const int left = K - k0 - E * lane;
+      if (E == 2) extra = lane < valid && shift(lane) && k0 + 63 < K ? word(after) : 0;
+#pragma unroll
+      for (int j = 0; j < kLoadRows; ++j, r += step)
+        a[j] = j < valid && left + static_cast<int>(E == 2 ? shift(j) >> 4 : 0) > 0 ? word(r) : 0;
+    }
+  }
+  // Whole warps: this lane's E elements of row j.
+  __device__ __forceinline__ uint32_t value(const uint32_t (&a)[kLoadRows], uint32_t extra, int j) const {
+    if constexpr (E == 1) return a[j];
+    const uint32_t last = __shfl_sync(0xffffffffu, extra, j), next = __shfl_down_sync(0xffffffffu, a[j], 1);
+    return __funnelshift_r(a[j], lane == 31 ? last : next, shift(j));
+  }
+  // Bits of this lane's elements of block k0 that are below K.
+  __device__ __forceinline__ uint32_t mask(int k0) const {
+    const int left = K - k0 - E * lane;
+    return E == 1 || left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
+  }
+};
+
+// The loading warps' loop over the nkb blocks of bk elements from block kb0 on:
+// `put(i, j, word)` stores a word of block i, row j of the warp; `ready(i)` waits
+// for block i's place in the ring and says whether to go on; `done(i)` hands it over.
+template <typename T, typename Ready, typename Put, typename Done>
+__device__ __forceinline__ void load_rows(const RowWords<T>& rows, int kb0, int nkb, int bk, Ready ready, Put put,
+                                          Done done) {
+  uint32_t a[kLoadRows], extra = 0;
+  rows.load(a, extra, kb0 * bk);
+  for (int i = 0; i < nkb; ++i) {
+    if (!ready(i)) return;
+    const int k0 = (kb0 + i) * bk;
+    const uint32_t mask = rows.mask(k0);
+#pragma unroll
+    for (int j = 0; j < kLoadRows; ++j) put(i, j, rows.value(a, extra, j) & mask);
+    if (i + 1 < nkb) rows.load(a, extra, k0 + bk);
+    done(i);
+  }
+}
+
+// TMEM columns [from, from + 16) of this thread's row into `total`'s (first: as
+// they are), added to nearest. Whole warps.
+__device__ __forceinline__ void tmem_add16(uint32_t total, uint32_t from, bool first) {
+  uint32_t v[16], t[16];
+  tmem_ld16(from, v);
+  if (!first) tmem_ld16(total, t);
+  tmem_ld_wait();
+  if (!first) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(t[i]) + __uint_as_float(v[i]));
+  }
+  tmem_st16(total, v);
+}
+
+// linear_sm100.cu. At most 64 rows, 16-byte rows of x and w (gemm_bf16_linear_takes).
 cudaError_t linear_skinny(const LinearArgs& g, bool out_bf16, cudaStream_t s);
-// Clusters of S CTAs (1 to 8, at most ceil(K / 64)) split K.
-cudaError_t linear_cluster(const LinearArgs& g, bool out_bf16, int S, int* status, cudaStream_t s);
+// Clusters of S CTAs (1 to 8, at most ceil(K / 64)) split K. `aligned`: 16-byte rows.
+cudaError_t linear_cluster(const LinearArgs& g, bool out_bf16, bool aligned, int S, int* status, cudaStream_t s);
 
 // linear_f32_sm100.cu: f32 operands; `takes`: 16-byte rows of x and w. S from 1
 // to 8, at most ceil(K / 32).
 bool linear_f32_takes(const LinearArgs& g);
-cudaError_t linear_f32(const LinearArgs& g, bool out_bf16, int S, int* status, cudaStream_t s);
+cudaError_t linear_f32(const LinearArgs& g, bool out_bf16, bool aligned, int S, int* status, cudaStream_t s);
 
 }  // namespace inl

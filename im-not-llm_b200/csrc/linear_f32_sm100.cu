@@ -14,6 +14,16 @@
 // linear_cluster_kernel. A sum that comes out NaN is computed again as a plain
 // f32 sum: the split turns an infinite (or rounding to infinity) operand into
 // inf - inf, and a row that holds one must still give what f32 gives.
+//
+// Bound by shared memory: a 128 x 128 x 32 block writes 32 KB (TMA), reads it,
+// writes 64 KB (hi, lo) and is read by 12 products of 8 KB, 224 KB or 1750 cycles
+// of the SM's 128 bytes a cycle, against 768 cycles of products. 1024 x 4096 x
+// 1024: 72 us = 120 TFLOP/s of f32 (an f32 library product: 162 us, off by
+// 5.7e-7 where this is off by 3.5e-7); 8192 x 1024 x 4096: 444 us; rows of odd
+// strides 92 and 561 us. With hi left to the tensor core's own truncation of
+// what TMA wrote 63 us, but an error of 6.3e-7, all of it toward zero.
+#include <type_traits>
+
 #include "../../include/inl_cuda.h"
 #include "../../include/inl_cuda_kernels.h"
 #include "common.cuh"
@@ -30,9 +40,8 @@ constexpr int kTile = kBM * kBK * 4;    // one operand's f32 tile
 constexpr int kStageBytes = 4 * kTile;  // x hi, w hi (in place of the loaded f32), x lo, w lo
 constexpr int kChunk = 4;               // K blocks between promotions of the large sum
 constexpr int kConvWarps = 4;
-constexpr int kThreads = 320 + 32 * kConvWarps;  // TMA, MMA, 8 sum warps, the splitting warps
 constexpr int kSmem = kStages * kStageBytes + 1024 + 256;
-constexpr int kTmemCols = 512;  // two large accumulators and the small one, 128 columns each (a power of two)
+constexpr int kTmemCols = 512;  // two large accumulators, the small one and a total, 128 columns each
 
 // Instruction descriptor of kind::tf32: D f32, A and B tf32, both K-major.
 __host__ __device__ constexpr uint32_t idesc_tf32(int M, int N) {
@@ -54,8 +63,12 @@ __device__ __forceinline__ float tf32_of(float x) {
   return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u);
 }
 
-template <typename TO>
-__global__ void __launch_bounds__(kThreads, 1)
+// TMA, MMA, 8 sum warps, the splitting warps; or, for rows that no TMA map
+// takes, sixteen warps that load them word by word and split them on the way.
+constexpr int threads_of(bool tma) { return 320 + 32 * (tma ? kConvWarps : kLoadWarps); }
+
+template <typename TO, bool TMA>
+__global__ void __launch_bounds__(threads_of(TMA), 1)
     linear_f32_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, LinearArgs g,
                       int S, int wide, int* status) {
   extern __shared__ uint8_t smem_raw[];
@@ -80,7 +93,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&split[s], kConvWarps);
+      mbar_init(&split[s], TMA ? kConvWarps : kLoadWarps);
       mbar_init(&empty[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
@@ -88,8 +101,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&tempty[a], 8);
     }
     fence_barrier_init();
-    tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmB);
+    if (TMA) {
+      tma_prefetch_desc(&tmA);
+      tma_prefetch_desc(&tmB);
+    }
   }
   if (warp == 1) {
     tmem_alloc(tmem_holder, kTmemCols);
@@ -102,7 +117,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (TMA && lane == 0) {
       int issued = 0;
       for (; issued < nkb; ++issued) {
         const int st = issued % kStages;
@@ -142,10 +157,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     // thread = tile row (lane quadrant warp % 4), 64 columns
     const int quad = warp & 3, half = (warp - 2) >> 2, row = quad * 32 + lane;
     const uint32_t t_row = tmem + (static_cast<uint32_t>(quad * 32) << 16) + half * 64;
-    float sum[64];
-#pragma unroll
-    for (int j = 0; j < 64; ++j) sum[j] = 0.f;
     const int chunks = (nkb + kChunk - 1) / kChunk;
+    // Sums in registers; in TMEM beside the loading warps, whose loads need them.
+    constexpr int R = TMA ? 64 : 16;
+    const uint32_t t_total = t_row + 3 * kBN;
+    float sum[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) sum[j] = 0.f;
     bool ok = true;
     for (int c = 0; c < chunks; ++c) {
       const int acc = c & 1;
@@ -153,31 +171,59 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
 #pragma unroll
       for (int j = 0; j < 64; j += 16) {
-        uint32_t r[16];
-        tmem_ld16(t_row + acc * kBN + j, r);
-        tmem_ld_wait();
+        if constexpr (TMA) {
+          uint32_t r[16];
+          tmem_ld16(t_row + acc * kBN + j, r);
+          tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum[j + i] += __uint_as_float(r[i]);
+          for (int i = 0; i < 16; ++i) sum[j + i] += __uint_as_float(r[i]);
+        } else {
+          tmem_add16(t_total + j, t_row + acc * kBN + j, c == 0);
+        }
       }
+      if constexpr (!TMA) tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&tempty[acc]);
     }
     if (ok) {
-#pragma unroll
-      for (int j = 0; j < 64; j += 16) {
-        uint32_t r[16];
-        tmem_ld16(t_row + 2 * kBN + j, r);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sum[j + i] += __uint_as_float(r[i]);
-      }
       // every product is done, so the ring's memory takes the partial tile
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        *reinterpret_cast<float4*>(cluster_piece<kBN>(smem, row, half * 16 + j)) =
-            make_float4(sum[4 * j], sum[4 * j + 1], sum[4 * j + 2], sum[4 * j + 3]);
+      for (int j = 0; j < 64; j += 16) {
+        uint32_t r[16], t[16];
+        tmem_ld16(t_row + 2 * kBN + j, r);
+        if constexpr (!TMA) tmem_ld16(t_total + j, t);
+        tmem_ld_wait();
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]) + (TMA ? sum[(j + i) % R] : __uint_as_float(t[i]));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<float4*>(cluster_piece<kBN>(smem, row, half * 16 + j / 4 + i)) =
+              make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      }
     }
+  } else if constexpr (!TMA) {
+    const int r0 = (warp - 10) * kLoadRows;  // of the stage's 256 rows: 128 of x, then 128 of w
+    const RowWords<float> rows = r0 < kBM ? RowWords<float>(g.x, g.ldx, m0 + r0, g.M, g.K, lane)
+                                          : RowWords<float>(g.w, g.ldw, n0 + r0 - kBM, g.N, g.K, lane);
+    load_rows(
+        rows, kb0, nkb, kBK,
+        [&](int i) {
+          return mbar_wait_warp(&empty[i % kStages], ((i / kStages) & 1) ^ 1, status, INL_DEV_TIMEOUT_PRODUCER);
+        },
+        [&](int i, int j, uint32_t word) {
+          const float v = __uint_as_float(word), h = tf32_of(v);
+          float* to = reinterpret_cast<float*>(smem + (i % kStages) * kStageBytes + (r0 + j) * 128 +
+                                               (((lane >> 2) ^ (j & 7)) << 4) + (lane & 3) * 4);
+          to[0] = h;
+          to[2 * kTile / 4] = v - h;
+        },
+        [&](int i) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&split[i % kStages]);
+        });
   } else {
     const int tid = threadIdx.x - 320;
     for (int i = 0; i < nkb; ++i) {
@@ -208,15 +254,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <typename TO>
+template <typename TO, bool TMA>
 cudaError_t launch_f32(const CUtensorMap& ta, const CUtensorMap& tb, const LinearArgs& g, int S, int wide, int* status,
                        cudaStream_t s) {
-  auto kern = linear_f32_kernel<TO>;
+  auto kern = linear_f32_kernel<TO, TMA>;
   static std::atomic<unsigned long long> attr_set{0};
   const cudaError_t err = set_smem_limit_once(kern, kSmem, attr_set);
   if (err != cudaSuccess) return err;
   const unsigned grid = ((g.M + kBM - 1) / kBM) * ((g.N + kBN - 1) / kBN) * S;
-  return launch_cluster_pdl(kern, grid, kThreads, kSmem, S, s, ta, tb, g, S, wide, status);
+  return launch_cluster_pdl(kern, grid, threads_of(TMA), kSmem, S, s, ta, tb, g, S, wide, status);
 }
 
 }  // namespace
@@ -228,15 +274,18 @@ bool linear_f32_takes(const LinearArgs& g) {
   return g.K > 0 && rows_ok(g.x, g.ldx, g.M) && rows_ok(g.w, g.ldw, g.N);
 }
 
-cudaError_t linear_f32(const LinearArgs& g, bool out_bf16, int S, int* status, cudaStream_t s) {
+cudaError_t linear_f32(const LinearArgs& g, bool out_bf16, bool aligned, int S, int* status, cudaStream_t s) {
   auto pad4 = [](long long n) { return (n + 3) & ~3ll; };
-  CUtensorMap ta, tb;
-  if (!make_tma_2d_f32(&ta, g.x, g.M, g.K, g.M == 1 ? pad4(g.K) : g.ldx, kBM, kBK) ||
-      !make_tma_2d_f32(&tb, g.w, g.N, g.K, g.N == 1 ? pad4(g.K) : g.ldw, kBN, kBK))
+  CUtensorMap ta = {}, tb = {};
+  if (aligned && (!make_tma_2d_f32(&ta, g.x, g.M, g.K, g.M == 1 ? pad4(g.K) : g.ldx, kBM, kBK) ||
+                  !make_tma_2d_f32(&tb, g.w, g.N, g.K, g.N == 1 ? pad4(g.K) : g.ldw, kBN, kBK)))
     return cudaErrorInvalidValue;
   const int wide = linear_wide(g, out_bf16);
-  return out_bf16 ? launch_f32<__nv_bfloat16>(ta, tb, g, S, wide, status, s)
-                  : launch_f32<float>(ta, tb, g, S, wide, status, s);
+  auto run = [&](auto tma) {
+    return out_bf16 ? launch_f32<__nv_bfloat16, decltype(tma)::value>(ta, tb, g, S, wide, status, s)
+                    : launch_f32<float, decltype(tma)::value>(ta, tb, g, S, wide, status, s);
+  };
+  return aligned ? run(std::true_type()) : run(std::false_type());
 }
 
 }  // namespace inl

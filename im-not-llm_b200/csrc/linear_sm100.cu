@@ -15,6 +15,7 @@
 // order, and runs the epilogue on it. No workspace, no atomics, the same bits
 // every time.
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/inl_cuda.h"
 #include "../../include/inl_cuda_kernels.h"
@@ -137,23 +138,30 @@ cudaError_t launch_skinny_for(const LinearArgs& g, cudaStream_t s) {
 
 // ------------------------------------------------------------------ cluster split-K
 constexpr int kBM = 128, kBK = 64;
-constexpr int kBN = 64;
-constexpr int kThreads = 320;  // warp 0 TMA, warp 1 MMA, warps 2..9 move the accumulator out
+// warp 0 TMA, warp 1 MMA, warps 2..9 move the accumulator out; for rows that no
+// TMA map takes, warps 10..25 load them
+constexpr int threads_of(bool tma) { return 320 + (tma ? 0 : 32 * kLoadWarps); }
 
+template <int kBN>
 struct ClusterCfg {
-  static constexpr int STAGES = 6;
+  static constexpr int STAGES = kBN == 128 ? 4 : 6;
   static constexpr int CHUNK = 8;  // K blocks (512 of K) between promotions of the sum
   static constexpr int A_BYTES = kBM * kBK * 2, B_BYTES = kBN * kBK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int PART_BYTES = kBM * kBN * 4;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + PART_BYTES + 1024 + 256;
 };
 
-template <typename TO>
-__global__ void __launch_bounds__(kThreads, 1)
+// TMA: 16-byte rows, tiles of 64 columns. Else rows of any alignment, loaded word
+// by word (RowWords) into the same swizzled layout, and tiles of 128 columns,
+// since those loads are what bounds it: 1024 x 4096 x 1024 at odd strides 48 us
+// (13 us aligned), 8192 x 1024 x 4096 272 us = 252 TFLOP/s. The same loads by
+// 4-byte cp.async took 268 and 1813 us.
+template <typename TO, bool TMA>
+__global__ void __launch_bounds__(threads_of(TMA), 1)
     linear_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                           LinearArgs g, int S, int wide, int* status) {
-  using C = ClusterCfg;
-  constexpr int BN = kBN;
+  constexpr int BN = TMA ? 64 : 128;
+  using C = ClusterCfg<BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -177,7 +185,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], TMA ? 1 : kLoadWarps);
       mbar_init(&empty[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
@@ -185,11 +193,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&tempty[a], 8);
     }
     fence_barrier_init();
-    tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmB);
+    if (TMA) {
+      tma_prefetch_desc(&tmA);
+      tma_prefetch_desc(&tmB);
+    }
   }
   if (warp == 1) {
-    tmem_alloc(tmem_holder, 2 * BN);
+    tmem_alloc(tmem_holder, TMA ? 2 * BN : 4 * BN);  // two accumulators (and a total: a power of two)
     tmem_relinquish();
   }
   tc_fence_before();
@@ -199,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (TMA && lane == 0) {
       int issued = 0;
       for (; issued < nkb; ++issued) {
         const int st = issued % C::STAGES, kb = kb0 + issued;
@@ -230,53 +240,103 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (i % C::CHUNK == C::CHUNK - 1 || i == nkb - 1) umma_commit(&tfull[acc]);
       }
     }
-  } else {
-    // thread = tile row (lane quadrant warp % 4), 32 columns. The tensor core's
-    // accumulator truncates (1e-6 of the sum, toward zero, by K = 1024): every
-    // CHUNK blocks it is moved out and summed here, rounded to nearest.
+  } else if (warp < 10) {
+    // thread = tile row (lane quadrant warp % 4), half of the columns. The
+    // tensor core's accumulator truncates (1e-6 of the sum, toward zero, by K =
+    // 1024): every CHUNK blocks it is moved out and summed here, rounded to
+    // nearest.
+    constexpr int HW = BN / 2;
     const int quad = warp & 3, half = (warp - 2) >> 2, row = quad * 32 + lane;
-    float sum[32];
+    const uint32_t t_row = tmem + (static_cast<uint32_t>(quad * 32) << 16) + half * HW;
+    // Sums in registers; in TMEM beside the loading warps, whose loads need them.
+    constexpr int R = TMA ? HW : 16;
+    float sum[R];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) sum[j] = 0.f;
+    for (int j = 0; j < R; ++j) sum[j] = 0.f;
     const int chunks = (nkb + C::CHUNK - 1) / C::CHUNK;
+    bool ok = true;
     for (int c = 0; c < chunks; ++c) {
       const int acc = c & 1;
-      if (!mbar_wait_warp(&tfull[acc], (c >> 1) & 1, status, INL_DEV_TIMEOUT_EPILOGUE)) break;
+      if (!(ok = mbar_wait_warp(&tfull[acc], (c >> 1) & 1, status, INL_DEV_TIMEOUT_EPILOGUE))) break;
       tc_fence_after();
-      uint32_t v[32];
-      tmem_ld32(tmem + (static_cast<uint32_t>(quad * 32) << 16) + acc * BN + half * 32, v);
-      tmem_ld_wait();
 #pragma unroll
-      for (int j = 0; j < 32; ++j) sum[j] += __uint_as_float(v[j]);
+      for (int j = 0; j < HW; j += 16) {
+        if constexpr (TMA) {
+          uint32_t v[16];
+          tmem_ld16(t_row + acc * BN + j, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum[j + i] += __uint_as_float(v[i]);
+        } else {
+          tmem_add16(t_row + 2 * BN + j, t_row + acc * BN + j, c == 0);
+        }
+      }
+      if constexpr (!TMA) tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&tempty[acc]);
     }
+    if (ok) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      *reinterpret_cast<float4*>(cluster_piece<BN>(part, row, half * 8 + j)) =
-          make_float4(sum[4 * j], sum[4 * j + 1], sum[4 * j + 2], sum[4 * j + 3]);
+      for (int j = 0; j < HW; j += 16) {
+        uint32_t t[16];
+        if constexpr (!TMA) {
+          tmem_ld16(t_row + 2 * BN + j, t);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float4 v;
+          if constexpr (TMA)
+            v = make_float4(sum[(j + 4 * i) % R], sum[(j + 4 * i + 1) % R], sum[(j + 4 * i + 2) % R], sum[(j + 4 * i + 3) % R]);
+          else
+            v = make_float4(__uint_as_float(t[4 * i]), __uint_as_float(t[4 * i + 1]), __uint_as_float(t[4 * i + 2]),
+                            __uint_as_float(t[4 * i + 3]));
+          *reinterpret_cast<float4*>(cluster_piece<BN>(part, row, half * (HW / 4) + j / 4 + i)) = v;
+        }
+      }
+    }
+  } else if constexpr (!TMA) {
+    const int r0 = (warp - 10) * kLoadRows;  // of the stage's 256 rows: 128 of x, then 128 of w
+    const RowWords<__nv_bfloat16> rows =
+        r0 < kBM ? RowWords<__nv_bfloat16>(g.x, g.ldx, m0 + r0, g.M, g.K, lane)
+                 : RowWords<__nv_bfloat16>(g.w, g.ldw, n0 + r0 - kBM, g.N, g.K, lane);
+    uint8_t* const to = r0 < kBM ? sA + r0 * 128 : sB + (r0 - kBM) * 128;
+    load_rows(
+        rows, kb0, nkb, kBK,
+        [&](int i) {
+          return mbar_wait_warp(&empty[i % C::STAGES], ((i / C::STAGES) & 1) ^ 1, status, INL_DEV_TIMEOUT_PRODUCER);
+        },
+        [&](int i, int j, uint32_t word) {  // A_BYTES = B_BYTES here
+          *reinterpret_cast<uint32_t*>(to + (i % C::STAGES) * C::A_BYTES + j * 128 + (((lane >> 2) ^ (j & 7)) << 4) +
+                                       (lane & 3) * 4) = word;
+        },
+        [&](int i) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[i % C::STAGES]);
+        });
   }
   tc_fence_before();
   cluster_sync_all();  // every partial tile is written
-  if (warp >= 2) cluster_finish<TO, kBN, false>(g, part, threadIdx.x - 64, rank, S, m0, n0, wide != 0);
+  if (warp >= 2 && warp < 10) cluster_finish<TO, BN, false>(g, part, threadIdx.x - 64, rank, S, m0, n0, wide != 0);
   cluster_sync_all();  // no CTA leaves while another may still read its partial tile
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 2 * BN);
+    tmem_dealloc(tmem, TMA ? 2 * BN : 4 * BN);
   }
 }
 
-template <typename TO>
+template <typename TO, bool TMA>
 cudaError_t launch_cluster(const CUtensorMap& ta, const CUtensorMap& tb, const LinearArgs& g, int S, int wide,
                            int* status, cudaStream_t s) {
-  using C = ClusterCfg;
-  auto kern = linear_cluster_kernel<TO>;
+  constexpr int BN = TMA ? 64 : 128;
+  auto kern = linear_cluster_kernel<TO, TMA>;
   static std::atomic<unsigned long long> attr_set{0};
-  cudaError_t err = set_smem_limit_once(kern, C::SMEM_BYTES, attr_set);
+  const cudaError_t err = set_smem_limit_once(kern, ClusterCfg<BN>::SMEM_BYTES, attr_set);
   if (err != cudaSuccess) return err;
-  const unsigned grid = ((g.M + kBM - 1) / kBM) * ((g.N + kBN - 1) / kBN) * S;
-  return launch_cluster_pdl(kern, grid, kThreads, C::SMEM_BYTES, S, s, ta, tb, g, S, wide, status);
+  const unsigned grid = ((g.M + kBM - 1) / kBM) * ((g.N + BN - 1) / BN) * S;
+  return launch_cluster_pdl(kern, grid, threads_of(TMA), ClusterCfg<BN>::SMEM_BYTES, S, s, ta, tb, g, S, wide, status);
 }
 
 }  // namespace
@@ -285,15 +345,18 @@ cudaError_t linear_skinny(const LinearArgs& g, bool out_bf16, cudaStream_t s) {
   return out_bf16 ? launch_skinny_for<__nv_bfloat16>(g, s) : launch_skinny_for<float>(g, s);
 }
 
-cudaError_t linear_cluster(const LinearArgs& g, bool out_bf16, int S, int* status, cudaStream_t s) {
+cudaError_t linear_cluster(const LinearArgs& g, bool out_bf16, bool aligned, int S, int* status, cudaStream_t s) {
   auto pad8 = [](long long n) { return (n + 7) & ~7ll; };
-  CUtensorMap ta, tb;
-  if (!make_tma_2d_bf16(&ta, g.x, g.M, g.K, g.M == 1 ? pad8(g.K) : g.ldx, kBM, kBK) ||
-      !make_tma_2d_bf16(&tb, g.w, g.N, g.K, g.N == 1 ? pad8(g.K) : g.ldw, kBN, kBK))
+  CUtensorMap ta = {}, tb = {};
+  if (aligned && (!make_tma_2d_bf16(&ta, g.x, g.M, g.K, g.M == 1 ? pad8(g.K) : g.ldx, kBM, kBK) ||
+                  !make_tma_2d_bf16(&tb, g.w, g.N, g.K, g.N == 1 ? pad8(g.K) : g.ldw, 64, kBK)))
     return cudaErrorInvalidValue;
   const int wide = linear_wide(g, out_bf16);
-  return out_bf16 ? launch_cluster<__nv_bfloat16>(ta, tb, g, S, wide, status, s)
-                  : launch_cluster<float>(ta, tb, g, S, wide, status, s);
+  auto run = [&](auto tma) {
+    return out_bf16 ? launch_cluster<__nv_bfloat16, decltype(tma)::value>(ta, tb, g, S, wide, status, s)
+                    : launch_cluster<float, decltype(tma)::value>(ta, tb, g, S, wide, status, s);
+  };
+  return aligned ? run(std::true_type()) : run(std::false_type());
 }
 
 }  // namespace inl
