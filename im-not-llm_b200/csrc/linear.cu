@@ -121,19 +121,21 @@ int cluster_size(const LinearArgs& g, int sms) {
   return tiles * 2 <= sms && k_blocks >= 6 ? 2 : 1;
 }
 
-// The same for the kernels whose CTAs take one 128 x 128 tile each (f32, and
-// rows of any alignment): the S of the least (waves over the SMs) x (blocks of
-// 128 bytes of k + 4 for a tile's start and end).
-// Measured (us), f32, S = 1 / 2 / 4 / 8: 1024 x 1024 x 1024 36 / 21 / 29 / 74;
-// 1024 x 4096 x 1024 72 / 85 / 117 / 262; 8192 x 1024 x 4096 478 / 444 / 575 /
-// 906; 4253 x 768 x 768 66 / 58 / 94 / 201; 32 x 1024 x 1024 40 / 22 / 15 / 12.
-int tile_cluster_size(const LinearArgs& g, int bk, int sms) {
+// The same for the kernels with 128 x 128 tiles (f32, and rows of any
+// alignment): the S of the least (waves over the SMs) x (blocks of 128 bytes of k
+// + 10 for a tile's start and end), the 10 once where a CTA walks over tiles
+// (f32, 16-byte rows, S = 1). Measured (us), f32, S = 1 / 2 / 4 / 8: 1024 x 1024 x
+// 1024 31 / 19 / 28 / 72; 1024 x 4096 x 1024 56 / 77 / 110 / 254; 8192 x 1024 x
+// 4096 385 / 386 / 501 / 816; 4253 x 768 x 768 44 / 49 / 84 / 194;
+// 128 x 1024 x 1024 30 / 18 / 13 / 15.
+int tile_cluster_size(const LinearArgs& g, int bk, bool walk, int sms) {
   const long long tiles = static_cast<long long>((g.M + 127) / 128) * ((g.N + 127) / 128);
   const int k_blocks = (g.K + bk - 1) / bk;
   int best = 1;
   long long least = -1;
-  for (int S = 1; S <= 8 && S <= k_blocks; S *= 2) {
-    const long long cost = (tiles * S + sms - 1) / sms * ((k_blocks + S - 1) / S + 4);
+  for (int S = 1; S <= 4 && S <= k_blocks; S *= 2) {
+    const long long waves = (tiles * S + sms - 1) / sms, blocks = (k_blocks + S - 1) / S;
+    const long long cost = walk && S == 1 ? waves * blocks + 10 : waves * (blocks + 10);
     if (least < 0 || cost < least) least = cost, best = S;
   }
   return best;
@@ -183,8 +185,8 @@ int linear(const LinearArgs& g, int dtype, int out_dtype, int* status, cudaStrea
   // bf16 rows of odd strides: 8 x 1024 5.0 / 10.8; 32 x 1024 15 / 12.
   if (g.K == 0 || g.M <= 8 || (g.M <= 16 && g.N <= 8 * sms))
     return launched("linear", linear_rows(g, xb, ob, aligned, s));
-  if (xb) return launched("linear", linear_cluster(g, ob, false, tile_cluster_size(g, 64, sms), status, s));
-  return launched("linear", linear_f32(g, ob, aligned, tile_cluster_size(g, 32, sms), status, s));
+  if (xb) return launched("linear", linear_cluster(g, ob, false, tile_cluster_size(g, 64, false, sms), status, s));
+  return launched("linear", linear_f32(g, ob, aligned, tile_cluster_size(g, 32, aligned, sms), status, s));
 }
 
 }  // namespace

@@ -183,6 +183,14 @@ __device__ __forceinline__ float plain_dot(const LinearArgs& g, long long m, lon
   return s;
 }
 
+// The NaNs among the sums v of row m, columns n .. n + 3, again.
+__device__ __forceinline__ void redo4(const LinearArgs& g, float4& v, long long m, int n) {
+  if (isnan(v.x)) v.x = plain_dot(g, m, n);
+  if (isnan(v.y) && n + 1 < g.N) v.y = plain_dot(g, m, n + 1);
+  if (isnan(v.z) && n + 2 < g.N) v.z = plain_dot(g, m, n + 2);
+  if (isnan(v.w) && n + 3 < g.N) v.w = plain_dot(g, m, n + 3);
+}
+
 // After a cluster barrier: 256 threads (tid) of each of the S CTAs sum their
 // share of the tile over the cluster's partial tiles, in rank order, and run
 // the epilogue on it. A thread keeps one 4-column piece; the CTAs take its rows
@@ -218,16 +226,45 @@ __device__ __forceinline__ void cluster_finish(const LinearArgs& g, uint8_t* par
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (i >= count || !isnan(v[i].x + v[i].y + v[i].z + v[i].w)) continue;
-        const long long m = m0 + r0 + i * S * STEP;
-        if (isnan(v[i].x)) v[i].x = plain_dot(g, m, n);
-        if (isnan(v[i].y) && n + 1 < g.N) v[i].y = plain_dot(g, m, n + 1);
-        if (isnan(v[i].z) && n + 2 < g.N) v[i].z = plain_dot(g, m, n + 2);
-        if (isnan(v[i].w) && n + 3 < g.N) v[i].w = plain_dot(g, m, n + 3);
+        redo4(g, v[i], m0 + r0 + i * S * STEP, n);
       }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i].x += bias[0], v[i].y += bias[1], v[i].z += bias[2], v[i].w += bias[3];
     linear_finish_rows<TO, 4>(g, v, m0 + r0, S * STEP, count, n, wide);
+  }
+}
+
+// The epilogue of 32 rows x 32 columns (corner m, n) of one warp, thread = row, v
+// its sums: turned in the warp's 4 KB at `buf` so that a row's columns are
+// neighbouring lanes' (8 lanes of 4 columns, 4 rows at a time). A NaN is computed
+// again as a plain f32 sum. f32 operands.
+template <typename TO>
+__device__ __forceinline__ void warp_finish32(const LinearArgs& g, uint8_t* buf, const float* v, int m, int n, int lane,
+                                              bool wide) {
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    *reinterpret_cast<float4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+        make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  __syncwarp();
+  const int q = lane & 7, r0 = lane >> 3, col = n + 4 * q;
+  if (col >= g.N) return;
+  float b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b[i] = g.bias && col + i < g.N ? __ldg(g.bias + col + i) : 0.f;
+#pragma unroll 1
+  for (int r = r0; r < min(32, g.M - m); r += 16) {
+    const int count = min(4, (g.M - m - r + 3) / 4);
+    float4 t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int rr = r + 4 * i;
+      t[i] = *reinterpret_cast<const float4*>(buf + rr * 128 + ((q ^ (rr & 7)) << 4));
+      if (isnan(t[i].x + t[i].y + t[i].z + t[i].w) && i < count) redo4(g, t[i], m + rr, col);
+      t[i].x += b[0], t[i].y += b[1], t[i].z += b[2], t[i].w += b[3];
+    }
+    linear_finish_rows<TO, 4>(g, t, m + r, 4, count, col, wide);
   }
 }
 
