@@ -170,64 +170,20 @@ __device__ __forceinline__ float ss_bf16_32(const float (&v)[32]) {
 }
 
 // ------------------------------------------------------------------ linear epilogues
-// act(v) of 32 accumulators: one runtime switch per 32 columns instead of a
-// kernel per activation.
-template <typename TO>
+// act(v) of 32 accumulators, for a bf16 result: one runtime switch per 32
+// columns instead of a kernel per activation.
 __device__ __forceinline__ void linear_act(float (&v)[32], int act) {
   auto each = [&](auto f) {
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = f(v[j]);
   };
   switch (act) {
-    case INL_ACT_SILU: each([](float x) { return act_for<TO>(x, INL_ACT_SILU); }); break;
-    case INL_ACT_GELU_ERF: each([](float x) { return act_for<TO>(x, INL_ACT_GELU_ERF); }); break;
-    case INL_ACT_GELU_TANH: each([](float x) { return act_for<TO>(x, INL_ACT_GELU_TANH); }); break;
-    case INL_ACT_RELU: each([](float x) { return act_for<TO>(x, INL_ACT_RELU); }); break;
-    case INL_ACT_TANH: each([](float x) { return act_for<TO>(x, INL_ACT_TANH); }); break;
+    case INL_ACT_SILU: each([](float x) { return act_fast(x, INL_ACT_SILU); }); break;
+    case INL_ACT_GELU_ERF: each([](float x) { return act_fast(x, INL_ACT_GELU_ERF); }); break;
+    case INL_ACT_GELU_TANH: each([](float x) { return act_fast(x, INL_ACT_GELU_TANH); }); break;
+    case INL_ACT_RELU: each([](float x) { return act_fast(x, INL_ACT_RELU); }); break;
+    case INL_ACT_TANH: each([](float x) { return act_fast(x, INL_ACT_TANH); }); break;
     default: break;
-  }
-}
-
-// 32 rows x 32 columns of one warp (thread = row, v = its columns) to f32 or
-// unaligned bf16 rows: turned in the warp's 4 KB of shared memory (16-byte
-// piece j of row r at piece j ^ (r & 7): both sides free of bank conflicts) so
-// that neighbouring lanes write, and read the residual at, neighbouring
-// columns, whatever the rows' alignment. row0, col: the chunk's corner.
-template <typename TO, typename TR>
-__device__ __forceinline__ void turn_store32(uint8_t* buf, const float (&v)[32], const EpiArgs& e, TO* out,
-                                             const TR* resid, int row0, int col, int lane) {
-  __syncwarp();  // the chunk before has been read
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    *reinterpret_cast<float4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-        make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-  __syncwarp();
-  const int rows = min(32, e.M - row0);
-  if (sizeof(TO) == 4 && e.aligned && e.N - col >= 32) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 4 * i + (lane >> 3), j = lane & 7;
-      if (r >= rows) break;
-      float4 w = *reinterpret_cast<const float4*>(buf + r * 128 + ((j ^ (r & 7)) << 4));
-      if (resid) {
-        const float4 q = *reinterpret_cast<const float4*>(resid + (row0 + r) * e.ldr + col + 4 * j);
-        w.x += q.x, w.y += q.y, w.z += q.z, w.w += q.w;
-      }
-      *reinterpret_cast<float4*>(out + (row0 + r) * e.ldo + col + 4 * j) = w;
-    }
-  } else if (lane < e.N - col) {
-    const int off = lane >> 2;
-#pragma unroll 8
-    for (int r = 0; r < rows; ++r) {
-      float w = *reinterpret_cast<const float*>(buf + r * 128 + ((off ^ (r & 7)) << 4) + (lane & 3) * 4);
-      if constexpr (sizeof(TO) == 4) {
-        if (resid) w += resid[(row0 + r) * e.ldr + col + lane];
-        out[(row0 + r) * e.ldo + col + lane] = w;
-      } else {
-        if (resid) w += __bfloat162float(resid[(row0 + r) * e.ldr + col + lane]);
-        out[(row0 + r) * e.ldo + col + lane] = __float2bfloat16_rn(w);
-      }
-    }
   }
 }
 
@@ -249,25 +205,11 @@ __device__ __forceinline__ void linear_bias32(float (&v)[32], const EpiArgs& e, 
   }
 }
 
-// Activation, residual and store of 32 columns of this thread's row (bias included in v).
-template <bool F32>
-__device__ __forceinline__ void linear_store32(float (&v)[32], const EpiArgs& e, OutStage& st, int row, int col,
-                                               int lane) {
-  const int row0 = row - lane;
-  linear_act<std::conditional_t<F32, float, __nv_bfloat16>>(v, e.act);
-  if constexpr (F32) {
-    turn_store32(st.buf, v, e, static_cast<float*>(e.out), reinterpret_cast<const float*>(e.resid), row0, col, lane);
-  } else if (e.aligned) {
-    if (e.resid != nullptr && row < e.M) {
-      float rr[32];
-      load_row32_bf16(e.resid + static_cast<long long>(row) * e.ldr + col, rr, e.N - col);
-#pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] += rr[j];
-    }
-    stage_store32(st, v, col, row0, lane);
-  } else {
-    turn_store32(st.buf, v, e, static_cast<__nv_bfloat16*>(e.out), e.resid, row0, col, lane);
-  }
+// The linear epilogue's arguments in the form its other kernels take them in.
+__device__ __forceinline__ LinearArgs linear_args(const EpiArgs& e) {
+  LinearArgs g{};
+  g.bias = e.bias, g.resid = e.resid, g.out = e.out, g.ldr = e.ldr, g.ldo = e.ldo, g.M = e.M, g.N = e.N, g.act = e.act;
+  return g;
 }
 
 // One q or k head of width D in TMEM columns [c0, c0 + D) of this thread's row:
@@ -445,11 +387,26 @@ __device__ __forceinline__ void epilogue_tile(uint32_t t_row, int row, int n0, i
       const int col = n0 + half * HW + c;
       if (col >= e.N) break;  // warp-uniform
       tmem_ld32(t_row + half * HW + c, r);
-      linear_bias32(v, e, col);
-      tmem_ld_wait();
+      if (EPI == INL_EPI_LINEAR_BF16 && e.aligned) {
+        linear_bias32(v, e, col);
+        tmem_ld_wait();
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(r[j]);
-      linear_store32<EPI == INL_EPI_LINEAR_F32>(v, e, st, row, col, lane);
+        for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(r[j]);
+        linear_act(v, e.act);
+        if (e.resid != nullptr && row_ok) {
+          float rr[32];
+          load_row32_bf16(e.resid + static_cast<long long>(row) * e.ldr + col, rr, e.N - col);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += rr[j];
+        }
+        stage_store32(st, v, col, row0, lane);
+      } else {
+        using TO = std::conditional_t<EPI == INL_EPI_LINEAR_F32, float, __nv_bfloat16>;
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+        warp_finish32<TO, false>(linear_args(e), st.buf, v, row0, col, lane, e.aligned != 0);
+      }
     }
   } else {
 #pragma unroll 1
@@ -511,6 +468,45 @@ __device__ __forceinline__ void epilogue_tile(uint32_t t_row, int row, int n0, i
       }
     }
   }
+}
+
+// The epilogue of one tile whose sum comes in parts of K (INL_EPI_LINEAR_F32_LONG),
+// for one warp: this thread's row, half of the columns, summed in registers.
+// `taken(acc)` gives accumulator acc back. False: a wait ran out.
+template <int BN, typename Taken>
+__device__ __forceinline__ bool epilogue_long(uint32_t tmem, uint64_t* tfull, int& acc, uint32_t& acc_phase, int parts,
+                                              int row0, int n0, int half, const EpiArgs& e, OutStage& st, int lane,
+                                              int* status, Taken taken) {
+  constexpr int HW = BN / 2;
+  float sum[HW];
+#pragma unroll
+  for (int j = 0; j < HW; ++j) sum[j] = 0.f;
+  for (int p = 0; p < parts; ++p) {
+    if (!mbar_wait_warp(&tfull[acc], acc_phase, status, INL_DEV_TIMEOUT_EPILOGUE)) return false;
+    tc_fence_after();
+#pragma unroll
+    for (int c = 0; c < HW; c += 32) {
+      uint32_t r[32];
+      tmem_ld32(tmem + static_cast<uint32_t>(acc * BN + half * HW + c), r);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) sum[c + j] += __uint_as_float(r[j]);
+    }
+    tc_fence_before();
+    __syncwarp();
+    taken(acc);
+    if (++acc == 2) {
+      acc = 0;
+      acc_phase ^= 1;
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < HW; c += 32) {
+    const int col = n0 + half * HW + c;
+    if (col >= e.N || row0 >= e.M) break;  // warp-uniform
+    warp_finish32<float, false>(linear_args(e), st.buf, sum + c, row0, col, lane, e.aligned != 0);
+  }
+  return true;
 }
 
 template <int BN, int EPI, int ACT>
@@ -658,44 +654,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Unit w = unit_of(u, splits, k_blocks);
       const int mb = w.tile / n_tiles, nb = w.tile - (w.tile / n_tiles) * n_tiles;
       if constexpr (LONG) {
-        // this warp's half of the tile, summed in registers over the parts of K
-        constexpr int HW = BN / 2;
-        float sum[HW];
-#pragma unroll
-        for (int j = 0; j < HW; ++j) sum[j] = 0.f;
-        bool ok = true;
-        for (int kb = w.kb0; kb < w.kb1; kb += kLongBlocks) {
-          if (!(ok = mbar_wait_warp(&tfull[acc], acc_phase, status, INL_DEV_TIMEOUT_EPILOGUE))) break;
-          tc_fence_after();
-          const uint32_t t = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
-                             static_cast<uint32_t>(acc * BN + half * HW);
-#pragma unroll
-          for (int c = 0; c < HW; c += 32) {
-            uint32_t r[32];
-            tmem_ld32(t + c, r);
-            tmem_ld_wait();
-#pragma unroll
-            for (int j = 0; j < 32; ++j) sum[c + j] += __uint_as_float(r[j]);
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&tempty[acc]);
-          if (++acc == 2) {
-            acc = 0;
-            acc_phase ^= 1;
-          }
-        }
-        if (!ok) break;
-#pragma unroll
-        for (int c = 0; c < HW; c += 32) {
-          const int col = nb * BN + half * HW + c;
-          if (col >= N) break;  // warp-uniform
-          float v[32];
-          linear_bias32(v, e, col);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] += sum[c + j];
-          linear_store32<true>(v, e, st, mb * kBM + quad * 32 + lane, col, lane);
-        }
+        if (!epilogue_long<BN>(tmem_base + (static_cast<uint32_t>(quad * 32) << 16), tfull, acc, acc_phase,
+                               (k_blocks + kLongBlocks - 1) / kLongBlocks, mb * kBM + quad * 32, nb * BN, half, e, st,
+                               lane, status, [&](int a) {
+                                 if (lane == 0) mbar_arrive(&tempty[a]);
+                               }))
+          break;
         continue;
       }
       if (!mbar_wait_warp(&tfull[acc], acc_phase, status, INL_DEV_TIMEOUT_EPILOGUE)) break;
@@ -775,6 +739,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int k_blocks = (K + kBK - 1) / kBK;
   const int splits = e.splits > 1 ? e.splits : 1;
   const int num_units = num_tiles * splits;
+  constexpr bool LONG = EPI == INL_EPI_LINEAR_F32_LONG;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -849,38 +814,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       bool ok = true;
       for (int u = pair; u < num_units && ok; u += n_pairs) {
         const Unit w = unit_of(u, splits, k_blocks);
-        if (!mbar_wait(&tempty[acc], acc_phase ^ 1, status, INL_DEV_TIMEOUT_MMA)) break;
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * C::BN);
-        for (int kb = w.kb0; kb < w.kb1; ++kb) {
-          if (!mbar_wait(&full[stage], phase, status, INL_DEV_TIMEOUT_MMA)) {
+        int kb_first = w.kb0;
+        do {
+          const int kb_end = LONG ? min(w.kb1, kb_first + kLongBlocks) : w.kb1;
+          if (!mbar_wait(&tempty[acc], acc_phase ^ 1, status, INL_DEV_TIMEOUT_MMA)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          // Descriptors differ from the ring's base descriptors only in the
-          // start-address field (address >> 4, 14 bits; shared memory < 256 KB).
-          const uint64_t a_desc = a_desc0 + static_cast<uint64_t>((stage * C::A_BYTES) >> 4);
-          const uint64_t b_desc = b_desc0 + static_cast<uint64_t>((stage * C::B_BYTES) >> 4);
+          const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * C::BN);
+          for (int kb = kb_first; kb < kb_end; ++kb) {
+            if (!mbar_wait(&full[stage], phase, status, INL_DEV_TIMEOUT_MMA)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            // Descriptors differ from the ring's base descriptors only in the
+            // start-address field (address >> 4, 14 bits; shared memory < 256 KB).
+            const uint64_t a_desc = a_desc0 + static_cast<uint64_t>((stage * C::A_BYTES) >> 4);
+            const uint64_t b_desc = b_desc0 + static_cast<uint64_t>((stage * C::B_BYTES) >> 4);
 #pragma unroll
-          for (int kk = 0; kk < kBK / 16; ++kk) {
-            umma_bf16_pair(d_tmem, a_desc + static_cast<uint64_t>(kk * 2), b_desc + static_cast<uint64_t>(kk * 2), idesc,
-                           (kb != w.kb0 || kk != 0) ? 1u : 0u);
+            for (int kk = 0; kk < kBK / 16; ++kk) {
+              umma_bf16_pair(d_tmem, a_desc + static_cast<uint64_t>(kk * 2), b_desc + static_cast<uint64_t>(kk * 2),
+                             idesc, (kb != kb_first || kk != 0) ? 1u : 0u);
+            }
+            umma_commit_pair(smem_u32(&empty[stage]));
+            umma_commit_pair(empty_peer0 + static_cast<uint32_t>(stage * sizeof(uint64_t)));
+            if (++stage == C::STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
           }
-          umma_commit_pair(smem_u32(&empty[stage]));
-          umma_commit_pair(empty_peer0 + static_cast<uint32_t>(stage * sizeof(uint64_t)));
-          if (++stage == C::STAGES) {
-            stage = 0;
-            phase ^= 1;
+          if (!ok) break;
+          umma_commit_pair(smem_u32(&tfull[acc]));
+          umma_commit_pair(tfull_peer0 + static_cast<uint32_t>(acc * sizeof(uint64_t)));
+          if (++acc == 2) {
+            acc = 0;
+            acc_phase ^= 1;
           }
-        }
-        if (!ok) break;
-        umma_commit_pair(smem_u32(&tfull[acc]));
-        umma_commit_pair(tfull_peer0 + static_cast<uint32_t>(acc * sizeof(uint64_t)));
-        if (++acc == 2) {
-          acc = 0;
-          acc_phase ^= 1;
-        }
+          kb_first = kb_end;
+        } while (LONG && kb_first < w.kb1);
       }
     }
   } else {
@@ -894,6 +867,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int u = pair; u < num_units; u += n_pairs) {
       const Unit w = unit_of(u, splits, k_blocks);
       const int mb = w.tile / n_tiles, nb = w.tile - (w.tile / n_tiles) * n_tiles;
+      if constexpr (LONG) {
+        if (!epilogue_long<C::BN>(tmem_base + (static_cast<uint32_t>(quad * 32) << 16), tfull, acc, acc_phase,
+                                  (k_blocks + kLongBlocks - 1) / kLongBlocks,
+                                  mb * 2 * kBM + static_cast<int>(rank) * kBM + quad * 32, nb * C::BN, half, e, st,
+                                  lane, status, [&](int a) {
+                                    if (lane == 0)
+                                      mbar_arrive_cluster(tempty_lead0 + static_cast<uint32_t>(a * sizeof(uint64_t)));
+                                  }))
+          break;
+        continue;
+      }
       if (!mbar_wait_warp(&tfull[acc], acc_phase, status, INL_DEV_TIMEOUT_EPILOGUE)) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * C::BN);
@@ -1011,8 +995,7 @@ cudaError_t dispatch_act(int act, const CUtensorMap& ta, const CUtensorMap& tb, 
 template <int EPI>
 cudaError_t launch_linear(int bn, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& to, int M, int N,
                           int K, const EpiArgs& e, int* status, cudaStream_t s) {
-  if constexpr (EPI != INL_EPI_LINEAR_F32_LONG)
-    if (bn == 256) return launch_gemm_pair<EPI, 0>(ta, tb, to, M, N, K, e, status, 0, s);
+  if (bn == 256) return launch_gemm_pair<EPI, 0>(ta, tb, to, M, N, K, e, status, 0, s);
   return bn == 128 ? launch_gemm<128, EPI, 0>(ta, tb, to, M, N, K, e, status, 0, s)
                    : launch_gemm<64, EPI, 0>(ta, tb, to, M, N, K, e, status, 0, s);
 }
@@ -1199,10 +1182,9 @@ int gemm_bf16_linear(const GemmArgs& g, bool out_bf16, cudaStream_t stream) {
   // The tensor core's f32 accumulator truncates: a sum of K = 1024 products is
   // off by 1e-6 of itself toward zero, one of 4096 by 4.4e-6, which an f32
   // result shows. Past 512, such a sum is moved out every 512 of K and added in
-  // registers, rounded to nearest (5e-7 at any K; 64 registers a thread, so
-  // tiles of at most 128 columns).
+  // registers, rounded to nearest (5e-7 at any K).
   const bool parts = !out_bf16 && g.K > kLongBlocks * kBK;
-  const int bn = !parts && t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64;
+  const int bn = t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64;
   CUtensorMap ta, tb, to;
   if (!make_kmajor_map(&ta, g.A, g.M, g.K, lda, kBM)) return -2;
   if (!make_kmajor_map(&tb, g.W, g.N, g.K, ldw, bn == 256 ? 128 : bn)) return -2;

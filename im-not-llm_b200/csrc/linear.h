@@ -2,6 +2,7 @@
 // (linear.cu, linear_sm100.cu).
 #pragma once
 
+#include <type_traits>
 #include <utility>
 
 #include "../../include/inl_cuda_kernels.h"
@@ -236,35 +237,77 @@ __device__ __forceinline__ void cluster_finish(const LinearArgs& g, uint8_t* par
 }
 
 // The epilogue of 32 rows x 32 columns (corner m, n) of one warp, thread = row, v
-// its sums: turned in the warp's 4 KB at `buf` so that a row's columns are
-// neighbouring lanes' (8 lanes of 4 columns, 4 rows at a time). A NaN is computed
-// again as a plain f32 sum. f32 operands.
-template <typename TO>
+// its sums: turned in the warp's 4 KB at `buf` (16-byte piece j of row r at j ^ (r
+// & 7): no bank conflicts on either side) so that a row's columns are
+// neighbouring lanes': 4 columns to a lane and 4 rows at a time where `wide`, else
+// a column to a lane, so that rows of any alignment are read and written in
+// whole runs. REDO (f32 operands): a NaN is computed again as a plain f32 sum.
+template <typename TO, bool REDO>
 __device__ __forceinline__ void warp_finish32(const LinearArgs& g, uint8_t* buf, const float* v, int m, int n, int lane,
                                               bool wide) {
-  __syncwarp();
+  __syncwarp();  // what was there before has been read
 #pragma unroll
   for (int j = 0; j < 8; ++j)
     *reinterpret_cast<float4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) =
         make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
   __syncwarp();
-  const int q = lane & 7, r0 = lane >> 3, col = n + 4 * q;
-  if (col >= g.N) return;
-  float b[4];
+  const int rows = min(32, g.M - m);
+  if (wide || REDO) {
+    const int q = lane & 7, col = n + 4 * q;
+    if (col >= g.N) return;
+    float b[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) b[i] = g.bias && col + i < g.N ? __ldg(g.bias + col + i) : 0.f;
+    for (int i = 0; i < 4; ++i) b[i] = g.bias && col + i < g.N ? __ldg(g.bias + col + i) : 0.f;
 #pragma unroll 1
-  for (int r = r0; r < min(32, g.M - m); r += 16) {
-    const int count = min(4, (g.M - m - r + 3) / 4);
-    float4 t[4];
+    for (int r = lane >> 3; r < rows; r += 16) {
+      const int count = min(4, (rows - r + 3) / 4);
+      float4 t[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int rr = r + 4 * i;
-      t[i] = *reinterpret_cast<const float4*>(buf + rr * 128 + ((q ^ (rr & 7)) << 4));
-      if (isnan(t[i].x + t[i].y + t[i].z + t[i].w) && i < count) redo4(g, t[i], m + rr, col);
-      t[i].x += b[0], t[i].y += b[1], t[i].z += b[2], t[i].w += b[3];
+      for (int i = 0; i < 4; ++i) {
+        const int rr = r + 4 * i;
+        t[i] = *reinterpret_cast<const float4*>(buf + rr * 128 + ((q ^ (rr & 7)) << 4));
+        if (REDO && isnan(t[i].x + t[i].y + t[i].z + t[i].w) && i < count) redo4(g, t[i], m + rr, col);
+        t[i].x += b[0], t[i].y += b[1], t[i].z += b[2], t[i].w += b[3];
+      }
+      linear_finish_rows<TO, 4>(g, t, m + r, 4, count, col, wide);
     }
-    linear_finish_rows<TO, 4>(g, t, m + r, 4, count, col, wide);
+  } else {
+    const int col = n + lane;
+    if (col >= g.N) return;
+    const float b = g.bias ? __ldg(g.bias + col) : 0.f;
+    const TO* res = g.resid ? static_cast<const TO*>(g.resid) + m * g.ldr + col : nullptr;
+    TO* out = static_cast<TO*>(g.out) + m * g.ldo + col;
+    const uint8_t* from = buf + (lane & 3) * 4;
+    const int piece = lane >> 2;
+    // eight rows: their residuals are read before the first is stored
+    auto eight = [&](int r0, auto every) {
+      constexpr bool EVERY = decltype(every)::value;
+      float4 t[2];
+      float* w = reinterpret_cast<float*>(t);
+      float q[8];
+      if (res) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i, res += g.ldr) q[i] = EVERY || r0 + i < rows ? load_f(res) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        w[i] = *reinterpret_cast<const float*>(from + (r0 + i) * 128 + ((piece ^ i) << 4)) + b;
+      act_rows<TO, 2>(t, g.act);
+      if (res) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] += q[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i, out += g.ldo)
+        if (EVERY || r0 + i < rows) store_f(out, w[i]);
+    };
+    if (rows == 32) {
+#pragma unroll 1
+      for (int r0 = 0; r0 < 32; r0 += 8) eight(r0, std::true_type());
+    } else {
+#pragma unroll 1
+      for (int r0 = 0; r0 < rows; r0 += 8) eight(r0, std::false_type());
+    }
   }
 }
 

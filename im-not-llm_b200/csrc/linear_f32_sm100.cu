@@ -282,8 +282,8 @@ __global__ void __launch_bounds__(threads_of(TMA), 1)
           if (lane == 0) mbar_arrive(sempty);
           const int m = tile / n_tiles * kBM + quad * 32, n = tile % n_tiles * kBN + half * 64;
           if (m < g.M && n < g.N) {
-            warp_finish32<TO>(g, stage_out + (warp - 2) * 4096, sum, m, n, lane, wide != 0);
-            if (n + 32 < g.N) warp_finish32<TO>(g, stage_out + (warp - 2) * 4096, sum + 32, m, n + 32, lane, wide != 0);
+            warp_finish32<TO, true>(g, stage_out + (warp - 2) * 4096, sum, m, n, lane, wide != 0);
+            if (n + 32 < g.N) warp_finish32<TO, true>(g, stage_out + (warp - 2) * 4096, sum + 32, m, n + 32, lane, wide != 0);
           }
         }
       }
