@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(256) rotary_any_kernel(RotaryArgs a) {
       return v;
     };
     const int half = a.rot / 2;
-    const int pos = a.pos[t];
+    const int pos = half ? a.pos[t] : 0;
     for (int i = lane; i < half; i += 32) {
       const int ja = a.interleaved ? 2 * i : i, jb = a.interleaved ? 2 * i + 1 : i + half;
       float c, s;
@@ -448,7 +448,7 @@ int run_rotary(const char* what, int dtype, int norm, RotaryArgs& a, cudaStream_
   const int es = dtype == INL_DTYPE_BF16 ? 2 : 4;
   for (HeadSet& h : a.set)
     if (h.heads == 0) h.x = nullptr, h.out = nullptr, h.w = nullptr, h.b = nullptr;
-  if (a.rot == 0) a.inv_freq = nullptr;
+  if (a.rot == 0) a.inv_freq = nullptr, a.pos = nullptr;
   const std::initializer_list<HookPtr> ptrs = {
       {a.set[0].x, es, "q"},   {a.set[1].x, es, "k"},   {a.set[0].out, es, "q_out"}, {a.set[1].out, es, "k_out"},
       {a.set[0].w, 4, "qw"},   {a.set[0].b, 4, "qb"},   {a.set[1].w, 4, "kw"},       {a.set[1].b, 4, "kb"},

@@ -134,7 +134,8 @@ def test_refusals_need_no_gpu():
     for bad in (dict(dt=2), dict(odt=-1), dict(M=-1), dict(N=-1), dict(K=-1), dict(K=(1 << 30) + 1), dict(act=6),
                 dict(act=-1), dict(ldx=7), dict(ldw=7), dict(ldo=1), dict(resid=16, ldr=1), dict(ldx=1 << 41),
                 dict(x=17), dict(w=17), dict(out=17), dict(bias=18), dict(resid=19), dict(status=2),
-                dict(dt=F32, x=18), dict(odt=F32, out=18), dict(resid=16, ldr=4, ldo=2)):
+                dict(dt=F32, x=18), dict(odt=F32, out=18), dict(resid=16, ldr=4, ldo=2),
+                dict(M=1 << 29, N=1 << 29, ldo=1 << 29)):
         assert call(**bad) == INVALID, bad
         assert n.last_error().startswith("linear: ")
     for null in (dict(x=None), dict(w=None), dict(out=None)):
@@ -156,6 +157,21 @@ SHAPES = [(1, 1, 1), (1, 4096, 1024), (2, 7, 3), (5, 3, 0), (3, 33, 17), (8, 256
 @pytest.mark.parametrize("M,N,K", SHAPES)
 def test_shapes(gpu, M, N, K, dt):
     _one(M, N, K, dt, dt, "none", True, False)
+
+
+# sizes on both sides of each choice between the kernels, none of them a multiple of a tile
+CHOICES = [  # bf16: few rows, by columns; K shared by clusters of 4 and 2; tiles of 64, 128 and 256 columns, K to 512 and past
+    (16, 1180, 136), (9, 2000, 136), (16, 4100, 72), (3, 5000, 264), (32, 1100, 520), (20, 1999, 136), (30, 5001, 136),
+    (64, 1150, 328), (100, 1000, 1032), (250, 700, 400), (500, 2300, 320), (500, 2300, 776), (2000, 1000, 200),
+    (2000, 1000, 1000), (4200, 760, 520), (4200, 760, 264), (16, 1500, 300), (1900, 1490, 72), (1500, 1500, 1100)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,odt,odd", [(BF16, BF16, 0), (BF16, F32, 0), (F32, F32, 0), (F32, BF16, 0), (BF16, BF16, 1),
+                                        (F32, F32, 1)])
+@pytest.mark.parametrize("M,N,K", CHOICES)
+def test_every_choice_of_kernel(gpu, M, N, K, dt, odt, odd):
+    _one(M, N, K, dt, odt, "gelu_tanh", True, True, pad=(odd, odd * 3, odd, 5 * odd), seed=21)
 
 
 @pytest.mark.gpu
@@ -194,12 +210,12 @@ def test_out_may_be_the_residual(gpu, dt, odt, M):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", [BF16, F32])
-@pytest.mark.parametrize("M", [1, 24, 140])
-def test_values_that_are_not_finite_stay_in_their_rows(gpu, M, dt):
+@pytest.mark.parametrize("M,N", [(1, 264), (24, 264), (140, 264), (2000, 1500)])
+def test_values_that_are_not_finite_stay_in_their_rows(gpu, M, N, dt):
     import torch
 
     n = _n()
-    N, K = 264, 136
+    K = 136
     x, _ = _rows(torch, M, K, 0, dt, 3)
     w, _ = _rows(torch, N, K, 0, dt, 4, 0.1)
     x[0, 5] = float("inf")
@@ -253,6 +269,28 @@ def test_captured_on_another_stream_and_replayed(gpu, dt, odt):
                 n.check(_call(n, torch, x, w, dt, odt, "silu", b, None, o), "linear")
         torch.cuda.synchronize()
         assert all(torch.equal(o, out) for o in outs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_rows_past_32_bit_offsets(gpu, dt):
+    """Row strides of 2^20 elements over 2100 rows, of x, of the residual and of out: the same bits as of packed rows."""
+    import torch
+
+    n = _n()
+    M, N, K, ld = 2100, 264, 72, 1 << 20
+    x, _ = _rows(torch, M, K, 0, dt, 3)
+    w, _ = _rows(torch, N, K, 0, dt, 4, K ** -0.5)
+    r, _ = _rows(torch, M, N, 0, dt, 5)
+    big = torch.zeros(M * ld, device="cuda", dtype=_dt(torch, dt)).view(M, ld)
+    xb, rb, ob = big[:, :K], big[:, 1024:1024 + N], big[:, 2048:2048 + N]
+    xb.copy_(x)
+    rb.copy_(r)
+    out = torch.empty(M, N, device="cuda", dtype=x.dtype)
+    n.check(_call(n, torch, x, w, dt, dt, "silu", None, r, out), "linear")
+    n.check(_call(n, torch, xb, w, dt, dt, "silu", None, rb, ob), "linear")
+    torch.cuda.synchronize()
+    assert torch.equal(ob, out) and (big[:, 2048 + N:2048 + N + 64] == 0).all()
 
 
 @pytest.mark.gpu

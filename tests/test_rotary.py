@@ -265,6 +265,73 @@ def test_rope(gpu, d, rot, inter, dt):
         assert torch.equal(frame[~inside], before[~inside])
 
 
+# many tokens of few heads (several tokens to a warp), of many (runs of heads), and more than the warps at once
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("T,heads,d,rot,inter", [(2500, 1, 64, 64, 0), (5003, 3, 80, 40, 0), (12001, 4, 64, 32, 1),
+                                                 (12001, 1, 128, 128, 0), (5003, 24, 128, 128, 0), (4999, 2, 256, 64, 0),
+                                                 (600, 70, 64, 64, 1), (9001, 2, 20, 10, 0), (3001, 1, 8, 8, 0)])
+def test_rope_of_many_tokens(gpu, T, heads, d, rot, inter, dt):
+    import torch
+
+    n = _n()
+    x = _rows(torch, T, heads * d, 8, 0, dt, T)
+    pos = torch.randint(0, 100000, (T,), generator=torch.Generator().manual_seed(T)).int().cuda()
+    freq = _freqs(torch, rot, 5e5)
+    frame, out, inside = _frame(torch, T, heads * d, 8, 0, dt)
+    n.check(_rope(n, torch, x, T, heads, d, rot, inter, pos, freq, 1.1, 0, out, dt), "rope")
+    torch.cuda.synchronize()
+    y = x[:, :heads * d].double().unflatten(-1, (heads, d))
+    want, mag = _rot64(torch, y, pos, freq, 1.1, rot, inter)
+    _assert_close(torch, out[:, :heads * d].unflatten(-1, (heads, d)), want, 8 * U * mag, dt)
+    assert (frame[~inside] == -55).all()
+    n.check(_rope(n, torch, x, T, heads, d, rot, inter, pos, freq, 1.1, 0, x, dt), "rope")  # in place
+    torch.cuda.synchronize()
+    assert torch.equal(x[:, :heads * d], out[:, :heads * d])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("T,hq,hkv,d,rot,inter,ln", [(5003, 2, 1, 64, 64, 0, 0), (12001, 3, 1, 80, 80, 0, 1),
+                                                     (9001, 1, 1, 128, 64, 1, 0), (5003, 16, 8, 128, 128, 0, 0),
+                                                     (4999, 8, 2, 256, 64, 0, 0), (700, 40, 8, 64, 64, 0, 1)])
+def test_qk_of_many_tokens(gpu, T, hq, hkv, d, rot, inter, ln, dt):
+    import torch
+
+    n = _n()
+    c = dict(hq=hq, hkv=hkv, d=d, rot=rot, inter=inter, ln=ln, eps=1e-6)
+    x = _rows(torch, T, (hq + 2 * hkv) * d, 0, 0, dt, d + T, 3.0)
+    q, k = x[:, :hq * d], x[:, hq * d:(hq + hkv) * d]
+    g = torch.Generator().manual_seed(T)
+    qw, kw = ((1 + 0.3 * torch.randn(d, generator=g)).cuda() for _ in range(2))
+    qb, kb = ((0.2 * torch.randn(d, generator=g)).cuda() for _ in range(2)) if ln else (None, None)
+    pos = torch.randint(0, 40000, (T,), generator=g).int().cuda()
+    freq = _freqs(torch, rot, 1e6)
+    qo, ko = torch.empty(T, hq * d, device="cuda", dtype=x.dtype), torch.empty(T, hkv * d, device="cuda", dtype=x.dtype)
+    n.check(_qk(n, torch, c, q, k, d, qw, qb, kw, kb, pos, freq, 1.0, qo, ko, dt, T), "qk")
+    torch.cuda.synchronize()
+    for src, out, h, w, b in ((q, qo, hq, qw, qb), (k, ko, hkv, kw, kb)):
+        v, tol = _norm64(src.double().unflatten(-1, (h, d)), w, b, ln, 1e-6)
+        want, mag = _rot64(torch, v, pos, freq, 1.0, rot, inter)
+        _assert_close(torch, out.unflatten(-1, (h, d)), want, 8 * U * mag + _rot64(torch, tol, pos, freq, 1.0, rot, inter)[1],
+                      dt)
+
+
+@pytest.mark.gpu
+def test_nothing_rotated_reads_no_positions(gpu):
+    import torch
+
+    n = _n()
+    for d in (64, 7):  # both kernels
+        x = _rows(torch, 5, 3 * d, 0, 0, F32, d)
+        out = torch.empty_like(x)
+        s = torch.cuda.current_stream().cuda_stream
+        n.check(n.lib().inl_cuda_rope(x.data_ptr(), 3 * d, F32, 5, 3, d, 0, 0, None, None, 1.0, 0, out.data_ptr(), 3 * d, s),
+                "rope")
+        torch.cuda.synchronize()
+        assert torch.equal(out, x)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("inter", [0, 1])
 def test_far_positions_keep_their_digits(gpu, inter):
