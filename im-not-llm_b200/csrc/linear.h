@@ -1,5 +1,5 @@
 // The linear layer's arguments and epilogue, shared by its kernels
-// (linear.cu, linear_sm100.cu).
+// (linear.cu, linear_sm100.cu, linear_f32_sm100.cu, gemm_sm100.cu).
 #pragma once
 
 #include <type_traits>
@@ -343,8 +343,8 @@ cudaError_t launch_cluster_pdl(void (*kern)(Params...), unsigned grid, int threa
 
 // ------------------------------------------------------------------ rows of any alignment
 // Sixteen warps fetch a stage of 256 rows (128 of x, 128 of w) x 128 bytes of K,
-// 16 rows each, a 4-byte word to a lane, into registers, two stages ahead (64 KB
-// in flight per SM).
+// 16 rows each, a 4-byte word to a lane, into registers, a stage ahead. (Two
+// ahead, or 32 rows to each of eight warps, spilled: the words are the registers.)
 constexpr int kLoadWarps = 16, kLoadRows = 256 / kLoadWarps;
 
 // One loading warp's rows. A bf16 row may start in the middle of a word: then
@@ -438,11 +438,11 @@ __device__ __forceinline__ void tmem_add16(uint32_t total, uint32_t from, bool f
 
 // linear_sm100.cu. At most 64 rows, 16-byte rows of x and w (gemm_bf16_linear_takes).
 cudaError_t linear_skinny(const LinearArgs& g, bool out_bf16, cudaStream_t s);
-// Clusters of S CTAs (1 to 8, at most ceil(K / 64)) split K. `aligned`: 16-byte rows.
+// Clusters of S CTAs (1, 2 or 4, at most ceil(K / 64)) split K. `aligned`: 16-byte rows.
 cudaError_t linear_cluster(const LinearArgs& g, bool out_bf16, bool aligned, int S, int* status, cudaStream_t s);
 
-// linear_f32_sm100.cu: f32 operands; `takes`: 16-byte rows of x and w. S from 1
-// to 8, at most ceil(K / 32).
+// linear_f32_sm100.cu: f32 operands; `takes`: 16-byte rows of x and w. S 1, 2 or
+// 4, at most ceil(K / 32).
 bool linear_f32_takes(const LinearArgs& g);
 cudaError_t linear_f32(const LinearArgs& g, bool out_bf16, bool aligned, int S, int* status, cudaStream_t s);
 

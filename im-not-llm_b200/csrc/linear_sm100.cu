@@ -5,15 +5,17 @@
 // from global memory straight into mma.sync fragments, with no shared memory
 // in between: the k order inside a product is free as long as x and w agree, so
 // a lane takes 16 contiguous bytes of its row as the k pairs (0,1 | 8,9) of one
-// m16n8k16 and of the next. A CTA owns 8 NT rows of w, its 8 warps split K and
-// are summed in shared memory in warp order.
+// m16n8k16 and of the next. A CTA owns 8 NT rows of w, its 8 or 16 warps split K
+// and are summed in shared memory in warp order. A read of w bounds it: one row x
+// 4096 x 1024 3.2 us = 2.6 TB/s, of which launch and one trip to memory are 2.
 //
 // linear_cluster_kernel: some hundreds of rows, or few columns. A cluster of S
 // CTAs shares one 128 x 64 tile, each with its own slice of K on tcgen05
 // (TMA ring, accumulator in TMEM); the partial tiles meet in shared memory and
 // every CTA sums its share of the elements over the cluster's copies, in rank
 // order, and runs the epilogue on it. No workspace, no atomics, the same bits
-// every time.
+// every time. 256 x 1024 x 2048: 8.0 us where the persistent kernel's 32 tiles
+// take 11.9.
 #include <algorithm>
 #include <type_traits>
 

@@ -425,10 +425,10 @@ int check_rotary(const char* what, int dtype, int T, int d, int rot, const Rotar
   if (rot < 0 || rot > d || (rot & 1)) return bad(what, "rotary_dim is even and at most d");
   if (!std::isfinite(a.scale)) return bad(what, "scale is finite");
   for (const HeadSet& h : a.set) {
-    if (h.heads < 0) return bad(what, "heads >= 0");
+    if (h.heads < 0 || h.heads > 65536) return bad(what, "heads from 0 to 65536");
     if (h.heads == 0 || T == 0) continue;
     if (h.hsx < d) return bad(what, "the head stride is at least d");
-    // 2^40 elements is above any device's memory and keeps the products in 64 bits
+    // 2^40 elements is above any device's memory and, with 2^16 heads, keeps the products in 64 bits
     if (h.hsx > (1ll << 40) || h.ldx > (1ll << 40) || h.ldo > (1ll << 40)) return bad(what, "strides below 2^40");
     if (T > 1 && (h.ldx < (h.heads - 1) * h.hsx + d || h.ldo < static_cast<long long>(h.heads) * d))
       return bad(what, "row strides are at least the row's width");

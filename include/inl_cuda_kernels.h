@@ -183,9 +183,12 @@ INL_API int inl_cuda_gated_delta_rule(const float* mixed, int64_t ld_mixed, cons
  * sums, bias, activation and residual in f32 and one rounding at the end.
  * `dtype` (INL_DTYPE_*) is that of x and w; `out_dtype` that of out and resid;
  * bias is f32; bias and resid may be NULL. act is any INL_ACT_*_. Any
- * M, N, K from 0 to 2^30 (K = 0: the product is zero), any row strides >= the
- * row length, element-aligned pointers; bf16 rows whose addresses are multiples of
- * 16 bytes (K, ldx, ldw multiples of 8) take the tcgen05 kernels. out may be
+ * M, N, K from 0 to 2^30 (K = 0: the product is zero; M * N up to 2^40), any
+ * row strides >= the row length, element-aligned pointers; rows of x and w on
+ * 16-byte boundaries are the fast case. f32 operands give f32 accuracy (they
+ * are split for the tensor cores, each to 2^-21 of itself or 2^-137, whichever is
+ * more; a sum that comes out NaN is computed again in plain f32, so infinities
+ * keep to their rows as they would). out may be
  * resid itself (same pointer and stride); it overlaps nothing else. Nothing
  * outside the [M, N] elements of out is written. `status` as for
  * inl_cuda_gemm_bf16. Memory must be reachable from the current device.
@@ -253,7 +256,7 @@ INL_API int inl_cuda_rope_frequencies(const inl_rope_config* config, double* inv
  * pair i being features (i, i + rotary_dim / 2), or (2i, 2i + 1) when
  * `interleaved`; the other features are copied. `inverse` rotates by -t (the
  * transpose: undoes a rotation of scale 1, and carries a gradient back).
- * T up to 2^30. pos: device int32 [T], any sign; inv_freq: device f64
+ * T up to 2^30, heads up to 65536. pos: device int32 [T], any sign; inv_freq: device f64
  * [rotary_dim / 2]; the angle is formed modulo one turn in 64 bits, so far
  * positions lose nothing and there is no table. out may be x itself (same pointer and
  * stride) and overlaps it in no other way. Element-aligned pointers, strides

@@ -144,7 +144,7 @@ def test_rope_refusals_need_no_gpu():
              ldo=64):
         return n.lib().inl_cuda_rope(x, ldx, dt, T, heads, d, rot, inter, pos, freq, scale, inv, out, ldo, None)
 
-    for bad in (dict(dt=2), dict(T=-1), dict(heads=-1), dict(d=0), dict(rot=31), dict(rot=34), dict(rot=-2),
+    for bad in (dict(dt=2), dict(T=-1), dict(T=(1 << 30) + 1), dict(heads=-1), dict(heads=65537, ldx=1 << 30, ldo=1 << 30), dict(d=0), dict(rot=31), dict(rot=34), dict(rot=-2),
                 dict(ldx=63), dict(ldo=63), dict(ldx=1 << 41), dict(scale=float("nan")), dict(scale=float("inf")),
                 dict(x=17), dict(out=33), dict(pos=18), dict(freq=20), dict(dt=F32, x=18),
                 dict(out=16, ldo=128)):
