@@ -76,7 +76,7 @@ struct EpiArgs {
   // linear epilogues
   const float* bias;
   int act;
-  int aligned;  // out and resid rows on 16-byte boundaries (bf16: out leaves by TMA), bias on a 16-byte boundary
+  int aligned;  // out and resid rows on 16-byte boundaries (bf16, ending on one too: out leaves by TMA), bias on one
 };
 
 // A work unit of the persistent schedule: a tile and the K blocks [kb0, kb1)
@@ -1168,6 +1168,9 @@ int gemm_bf16_linear(const GemmArgs& g, bool out_bf16, cudaStream_t stream) {
   auto on16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   auto ld_ok = [&](long long ld) { return g.M == 1 || (ld % per16 == 0 && ld * (16 / per16) < (1ll << 40)); };
   e.aligned = on16(g.out) && ld_ok(g.ldo) && (!g.resid || (on16(g.resid) && ld_ok(g.ldr))) && on16(g.bias);
+  // a TMA store writes whole 16-byte pieces: a row that ends inside one would
+  // take the columns behind it along
+  if (out_bf16 && g.N % 8 != 0) e.aligned = 0;
   // The tile that finishes first by (waves over the SMs) x (time of a tile): at
   // K = 1024 a 256 x 256 tile of a CTA pair takes 7.2 us, a 128 x 128 tile 5.0,
   // a 128 x 64 tile 4.6 in a long run, and 8 : 6 : 5 where there is one wave.
@@ -1190,7 +1193,7 @@ int gemm_bf16_linear(const GemmArgs& g, bool out_bf16, cudaStream_t stream) {
   if (!make_kmajor_map(&tb, g.W, g.N, g.K, ldw, bn == 256 ? 128 : bn)) return -2;
   std::memset(&to, 0, sizeof(to));
   if (out_bf16 && e.aligned &&
-      !make_tma_2d_bf16_swizzled(&to, g.out, g.M, g.N, g.M == 1 ? pad8(g.N) : g.ldo, 32, 32, 64))
+      !make_tma_2d_bf16_swizzled(&to, g.out, g.M, g.N, g.M == 1 ? g.N : g.ldo, 32, 32, 64))
     return -2;
   const cudaError_t err =
       out_bf16 ? launch_linear<INL_EPI_LINEAR_BF16>(bn, ta, tb, to, g.M, g.N, g.K, e, g.status, stream)

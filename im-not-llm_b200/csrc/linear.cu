@@ -155,6 +155,7 @@ int linear(const LinearArgs& g, int dtype, int out_dtype, int* status, cudaStrea
   if ((g.M > 1 && (g.ldx < g.K || g.ldo < g.N || (g.resid && g.ldr < g.N))) || (g.N > 1 && g.ldw < g.K))
     return bad("row strides are at least the row's width");
   if (!g.out || (g.K > 0 && (!g.x || !g.w))) return record_error(INL_ERR_CONFIG, "linear: NULL x, w or out");
+  if (g.K > 0 && (g.out == g.x || g.out == g.w)) return bad("out is neither x nor w");
   if (g.resid == g.out && g.M > 1 && g.ldr != g.ldo) return bad("out may be resid only at the same stride");
   const int es = dtype == INL_DTYPE_BF16 ? 2 : 4, eo = out_dtype == INL_DTYPE_BF16 ? 2 : 4;
   const std::initializer_list<HookPtr> ptrs = {{g.K ? g.x : nullptr, es, "x"}, {g.K ? g.w : nullptr, es, "w"},

@@ -127,14 +127,14 @@ def test_refusals_need_no_gpu():
     n = _n()
     f = n.lib().inl_cuda_linear
 
-    def call(x=16, ldx=8, w=16, ldw=8, dt=BF16, M=2, N=2, K=8, bias=None, act=3, resid=None, ldr=2, out=16, ldo=2,
+    def call(x=16, ldx=8, w=64, ldw=8, dt=BF16, M=2, N=2, K=8, bias=None, act=3, resid=None, ldr=2, out=128, ldo=2,
              odt=BF16, status=None):
         return f(x, ldx, w, ldw, dt, M, N, K, bias, act, resid, ldr, out, ldo, odt, status, None)
 
     for bad in (dict(dt=2), dict(odt=-1), dict(M=-1), dict(N=-1), dict(K=-1), dict(K=(1 << 30) + 1), dict(act=6),
                 dict(act=-1), dict(ldx=7), dict(ldw=7), dict(ldo=1), dict(resid=16, ldr=1), dict(ldx=1 << 41),
-                dict(x=17), dict(w=17), dict(out=17), dict(bias=18), dict(resid=19), dict(status=2),
-                dict(dt=F32, x=18), dict(odt=F32, out=18), dict(resid=16, ldr=4, ldo=2),
+                dict(x=17), dict(w=17), dict(out=17), dict(out=16), dict(out=64), dict(bias=18), dict(resid=19), dict(status=2),
+                dict(dt=F32, x=18), dict(odt=F32, out=18), dict(resid=128, ldr=4, ldo=2),
                 dict(M=1 << 29, N=1 << 29, ldo=1 << 29)):
         assert call(**bad) == INVALID, bad
         assert n.last_error().startswith("linear: ")
@@ -190,6 +190,13 @@ def test_epilogues(gpu, act, dt, odt, M):
                                         ((0, 0, 0, 7), 0), ((8, 8, 8, 8), 1), ((5, 7, 9, 11), 3)])
 def test_strides_and_alignment(gpu, M, N, K, pad, offset, dt, odt):
     _one(M, N, K, dt, odt, "silu", True, True, pad, offset, seed=9)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,odt", [(BF16, BF16), (BF16, F32), (F32, F32), (F32, BF16)])
+@pytest.mark.parametrize("M,N,K", [(806, 5, 248), (300, 773, 776), (2000, 1003, 72), (4200, 757, 264), (70, 1001, 1032)])
+def test_columns_behind_a_row_that_ends_inside_16_bytes_stay(gpu, M, N, K, dt, odt):
+    _one(M, N, K, dt, odt, "none", True, False, pad=(8, 8, 0, -N % 8), offset=8)
 
 
 @pytest.mark.gpu
