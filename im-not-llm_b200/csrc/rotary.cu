@@ -195,13 +195,14 @@ struct Vec {
 // heads, or of the next tokens) as soon as it has taken this one out of the
 // registers.
 //
-// Bound by memory: 65536 tokens of 24 bf16 heads of 128, rotated 124 us = 6.5
-// TB/s (all of a copy's rate), normed and rotated 145 us = 5.6 TB/s; 20011 f32
+// Bound by memory: 65536 tokens of 24 bf16 heads of 128, rotated 123 us = 6.5
+// TB/s (all of a copy's rate), normed and rotated 141 us = 5.7 TB/s; 20011 f32
 // tokens of 12 heads of 64, interleaved, 25 us = 5.0 TB/s. Tried on the first
 // of these (us): a block per 4 tokens, a barrier between its cos / sin and its
 // heads 175; blocks that walk over tiles, with that barrier 153 to 178; 2 / 4
 // heads in flight 137 / 187 (registers); 8-byte vectors 202; more resident
-// warps at fewer registers 149 and more.
+// warps at fewer registers 149 and more; two features to an instruction 125
+// (normed 143); a head's address made anew for each load 124 (normed 145).
 template <typename T, int E, int NORM, bool INTER, int KI>
 __global__ void __launch_bounds__(256, 2) rotary_vec_kernel(RotaryArgs a, int log_lanes, int log_tokens, int run) {
   using V = Vec<T, E>;
@@ -226,12 +227,18 @@ __global__ void __launch_bounds__(256, 2) rotary_vec_kernel(RotaryArgs a, int lo
   float4* const wsm = smem4 + 8 * cs_n;
   uint64_t* const steps = reinterpret_cast<uint64_t*>(wsm + (NORM == kNoNorm ? 0 : a.d));  // [half]
 
-  auto load = [&](int tile, int h, Raw (&raw)[2]) {
+  // A row's q heads and k heads, at this lane's features; the keys' pointer is
+  // set back by hq heads, so that head h of either lies h strides on.
+  const int hs_q = static_cast<int>(a.set[0].hsx), hs_k = static_cast<int>(a.set[1].hsx);
+  auto row_at = [&](int tile, const T*& q, const T*& k) {
     const long long row = min((tile << log_tokens) + tok, a.T - 1);
+    q = static_cast<const T*>(a.set[0].x) + row * a.set[0].ldx + f;
+    k = static_cast<const T*>(a.set[1].x) + row * a.set[1].ldx + (f - hq * hs_k);
+  };
+  auto load = [&](const T* q, const T* k, int h, Raw (&raw)[2]) {
     h = min(h, run1 - 1);
     const bool second = h >= hq;
-    const HeadSet& st = a.set[second];
-    const T* x = static_cast<const T*>(st.x) + row * st.ldx + static_cast<int>(second ? h - hq : h) * static_cast<int>(st.hsx) + f;
+    const T* x = (second ? k : q) + h * (second ? hs_k : hs_q);
     raw[0] = *reinterpret_cast<const Raw*>(x);
     raw[1] = *reinterpret_cast<const Raw*>(x + gap);
   };
@@ -245,9 +252,11 @@ __global__ void __launch_bounds__(256, 2) rotary_vec_kernel(RotaryArgs a, int lo
   const int tile_step = gridDim.x * 8;
   Raw raw[KI][2];
   int pos = 0;
+  const T *xq = nullptr, *xk = nullptr;
   if (tile < tiles) {
+    row_at(tile, xq, xk);
 #pragma unroll
-    for (int k = 0; k < KI; ++k) load(tile, h0 + k * step, raw[k]);
+    for (int k = 0; k < KI; ++k) load(xq, xk, h0 + k * step, raw[k]);
     pos = load_pos(tile);
   }
   for (int i = threadIdx.x; i < half; i += 256) steps[i] = turn_step(a.inv_freq[i]);
@@ -278,7 +287,11 @@ __global__ void __launch_bounds__(256, 2) rotary_vec_kernel(RotaryArgs a, int lo
             make_float2(co * a.scale, si * (a.scale * a.sin_sign));
       }
     }
-    if (next < tiles) pos = load_pos(next);
+    const T *nq = xq, *nk = xk;
+    if (next < tiles) {
+      pos = load_pos(next);
+      row_at(next, nq, nk);
+    }
     __syncwarp();
     float c[E], sn[E];
     if (turned) {
@@ -290,6 +303,8 @@ __global__ void __launch_bounds__(256, 2) rotary_vec_kernel(RotaryArgs a, int lo
     }
     const long long row = (tile << log_tokens) + tok;
     const bool mine = active && row < a.T;
+    T* const oq = static_cast<T*>(a.set[0].out) + row * a.set[0].ldo + f;
+    T* const ok = static_cast<T*>(a.set[1].out) + row * a.set[1].ldo + (f - hq * a.d);
     for (int b = 0; run0 + b < run1; b += KI * step) {
       const bool more = run0 + b + KI * step < run1;  // heads of this token after the batch
 #pragma unroll
@@ -299,7 +314,8 @@ __global__ void __launch_bounds__(256, 2) rotary_vec_kernel(RotaryArgs a, int lo
         float v[2 * E];
         V::unpack(raw[k][0], v);
         V::unpack(raw[k][1], v + E);
-        if (more || next < tiles) load(more ? tile : next, more ? h + KI * step : h0 + k * step, raw[k]);
+        if (more) load(xq, xk, h + KI * step, raw[k]);
+        else if (next < tiles) load(nq, nk, h0 + k * step, raw[k]);
         if (run0 + b + k * step >= run1) continue;  // the same for the whole warp
         if constexpr (NORM != kNoNorm) {
           const float rd = 1.f / static_cast<float>(a.d);
@@ -340,13 +356,13 @@ __global__ void __launch_bounds__(256, 2) rotary_vec_kernel(RotaryArgs a, int lo
           }
         }
         if (mine && h < run1) {
-          const HeadSet& st = a.set[second];
-          T* out = static_cast<T*>(st.out) + row * st.ldo + static_cast<int>(second ? h - hq : h) * a.d + f;
+          T* out = (second ? ok : oq) + h * a.d;
           *reinterpret_cast<Raw*>(out) = V::pack(v);
           *reinterpret_cast<Raw*>(out + gap) = V::pack(v + E);
         }
       }
     }
+    xq = nq, xk = nk;
   }
 }
 
@@ -380,13 +396,14 @@ cudaError_t launch_vec(const RotaryArgs& a, cudaStream_t s) {
 // Whether heads, pairs and rows come apart into E-vectors, 32 units to a head at most.
 bool vec_takes(const RotaryArgs& a, int E, int elem) {
   if (a.rot % (2 * E) || a.d % (2 * E) || a.d > 64 * E) return false;
+  const long long heads = static_cast<long long>(a.set[0].heads) + a.set[1].heads;
+  if (heads * a.d > INT_MAX) return false;  // 32-bit offsets inside a row, k's from hq heads before it
   for (const HeadSet& h : a.set) {
     if (h.heads == 0) continue;
     if ((reinterpret_cast<uintptr_t>(h.x) | reinterpret_cast<uintptr_t>(h.out)) % static_cast<unsigned>(E * elem))
       return false;
     if (a.T > 1 && (h.ldx % E || h.ldo % E)) return false;
-    if (h.heads > 1 && (h.hsx % E || h.hsx * h.heads > INT_MAX)) return false;  // 32-bit offsets inside a row
-    if (static_cast<long long>(h.heads) * a.d > INT_MAX) return false;
+    if (h.heads > 1 && (h.hsx % E || h.hsx * heads > INT_MAX)) return false;
   }
   return true;
 }
