@@ -18,6 +18,7 @@
 // Tiles are walked in row-major tile order by a static stride-gridDim
 // schedule, so the CTAs resident at one time share the same few X row blocks
 // and read W (a few MB) out of L2.
+#include <algorithm>
 #include <cstdio>
 #include <cstring>
 #include <type_traits>
@@ -38,11 +39,11 @@ constexpr int kLongBlocks = 8;  // K blocks between promotions of INL_EPI_LINEAR
 
 template <int BN>
 struct GemmCfg {
-  static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+  static constexpr int STAGES = BN >= 192 ? 4 : BN == 128 ? 6 : 8;
   static constexpr int A_BYTES = kBM * kBK * 2;
   static constexpr int B_BYTES = BN * kBK * 2;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int TMEM_COLS = 2 * BN;  // two accumulator buffers
+  static constexpr int TMEM_COLS = BN > 128 ? 512 : 2 * BN;  // two accumulator buffers, a power of two
   static constexpr int OUT_STAGE_BYTES = kEpiWarps * 2 * 32 * 64;  // per epilogue warp: 2 chunks of 32 x 32 bf16
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + OUT_STAGE_BYTES + 1024 /*align*/ + 256 /*barriers*/;
 };
@@ -995,7 +996,9 @@ cudaError_t dispatch_act(int act, const CUtensorMap& ta, const CUtensorMap& tb, 
 template <int EPI>
 cudaError_t launch_linear(int bn, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& to, int M, int N,
                           int K, const EpiArgs& e, int* status, cudaStream_t s) {
-  if (bn == 256) return launch_gemm_pair<EPI, 0>(ta, tb, to, M, N, K, e, status, 0, s);
+  if constexpr (EPI != INL_EPI_LINEAR_F32)
+    if (bn == 256) return launch_gemm_pair<EPI, 0>(ta, tb, to, M, N, K, e, status, 0, s);
+  if (bn == 192) return launch_gemm<192, EPI, 0>(ta, tb, to, M, N, K, e, status, 0, s);
   return bn == 128 ? launch_gemm<128, EPI, 0>(ta, tb, to, M, N, K, e, status, 0, s)
                    : launch_gemm<64, EPI, 0>(ta, tb, to, M, N, K, e, status, 0, s);
 }
@@ -1149,6 +1152,38 @@ int gemm_bf16_tn(const GemmArgs& g, cudaStream_t stream) {
   return err == cudaSuccess ? 0 : -3;
 }
 
+// Columns of the tile (256: a 256 x 256 tile of a CTA pair; 192, 128, 64: 128 rows
+// of one CTA) that finishes a linear layer first: the tiles' waves over the SMs
+// times the slower of a tile's products and its epilogue, and once the faster of
+// the two. us of a K block and of an epilogue, and per 64 columns of a residual,
+// fitted to 306 random sizes (256 to 131072 rows) x 4 tiles; over those the
+// choice is 0.4% slower than the best tile in the mean, 17% at most. Measured
+// (us), 256 / 192 / 128 / 64, bf16 with gelu: 4253 x 768 x 768 13.7 / 10.7 / 13.5
+// / 15.6; 4253 x 2304 x 768 27 / 21 / 27 / 39; 2048 x 1024 x 1024 14.4 / 11.9 /
+// 10.3 / 13.6; 8192 x 1024 x 2048 33 / 39 / 45 / 69; bf16 to f32: 4253 x 2304 x
+// 768 33 / 23 / 26 / 39; 16384 x 768 x 768 36 / 29 / 30 / 47.
+static int linear_tile(int M, int N, int K, int kind, bool resid) {
+  constexpr int cols[4] = {256, 192, 128, 64};
+  constexpr float block[4] = {0.40f, 0.35f, 0.32f, 0.30f};
+  constexpr float epilogue[4][4] = {{4.7f, 3.1f, 2.4f, 1.9f},    // bf16, no activation or relu
+                                    {5.7f, 4.1f, 2.9f, 1.6f},    // bf16, another activation
+                                    {0.0f, 4.0f, 3.1f, 1.6f},    // f32, K in one part
+                                    {14.9f, 6.6f, 4.3f, 3.3f}};  // f32, K in parts
+  const long long sms = num_sms();
+  const float k_blocks = static_cast<float>((K - 1) / kBK + 1);
+  int best = 0;
+  float least = 0.f;
+  for (int i = kind == 2 ? 1 : 0; i < 4; ++i) {  // there the pair's tile is never the first
+    const long long rows = i == 0 ? 2 * kBM : kBM, at_once = i == 0 ? sms / 2 : sms;
+    const long long tiles = ((M + rows - 1) / rows) * ((N + cols[i] - 1ll) / cols[i]);
+    const float products = block[i] * k_blocks;
+    const float out = epilogue[kind][i] + (resid ? (kind < 2 ? 0.6f : 1.0f) * static_cast<float>(cols[i] / 64) : 0.f);
+    const float time = static_cast<float>((tiles + at_once - 1) / at_once) * std::max(products, out) + std::min(products, out);
+    if (best == 0 || time < least) best = cols[i], least = time;
+  }
+  return best;
+}
+
 bool gemm_bf16_linear_takes(const GemmArgs& g) {
   // what a TMA map asks of x and w: 16-byte rows (K may end anywhere inside one)
   auto rows_ok = [](const void* p, long long ld, long long rows) {
@@ -1171,23 +1206,13 @@ int gemm_bf16_linear(const GemmArgs& g, bool out_bf16, cudaStream_t stream) {
   // a TMA store writes whole 16-byte pieces: a row that ends inside one would
   // take the columns behind it along
   if (out_bf16 && g.N % 8 != 0) e.aligned = 0;
-  // The tile that finishes first by (waves over the SMs) x (time of a tile): at
-  // K = 1024 a 256 x 256 tile of a CTA pair takes 7.2 us, a 128 x 128 tile 5.0,
-  // a 128 x 64 tile 4.6 in a long run, and 8 : 6 : 5 where there is one wave.
-  // Measured (us), pair / 128 / 64: 1024 x 1024 x 1024 11.2 / 8.7 / 8.1;
-  // 2048 x 1024 x 1024 11.4 / 8.9 / 12.8; 1024 x 4096 x 1024 12.2 / 14.2 / 22.1;
-  // 8192 x 1024 x 2048 28.9 / 40.8 / 65.4.
-  const long long sms = num_sms();
-  auto waves = [&](long long bm, long long bn, long long at_once) {
-    return ((g.M + bm - 1) / bm * ((g.N + bn - 1) / bn) + at_once - 1) / at_once;
-  };
-  const long long t256 = 8 * waves(256, 256, sms / 2), t128 = 6 * waves(128, 128, sms), t64 = 5 * waves(128, 64, sms);
   // The tensor core's f32 accumulator truncates: a sum of K = 1024 products is
   // off by 1e-6 of itself toward zero, one of 4096 by 4.4e-6, which an f32
   // result shows. Past 512, such a sum is moved out every 512 of K and added in
   // registers, rounded to nearest (5e-7 at any K).
   const bool parts = !out_bf16 && g.K > kLongBlocks * kBK;
-  const int bn = t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64;
+  const bool plain = g.act == INL_ACT_NONE_ || g.act == INL_ACT_RELU_;
+  const int bn = linear_tile(g.M, g.N, g.K, out_bf16 ? (plain ? 0 : 1) : (parts ? 3 : 2), g.resid != nullptr);
   CUtensorMap ta, tb, to;
   if (!make_kmajor_map(&ta, g.A, g.M, g.K, lda, kBM)) return -2;
   if (!make_kmajor_map(&tb, g.W, g.N, g.K, ldw, bn == 256 ? 128 : bn)) return -2;
