@@ -176,12 +176,14 @@ def test_every_choice_of_kernel(gpu, M, N, K, dt, odt, odd):
 
 # the persistent product's tiles: 64, 128 and 192 columns and the pair's 256, K in one part and in several
 TILES = [(500, 2300, 392), (500, 2300, 1096), (2000, 1000, 72), (2000, 1000, 520), (4200, 760, 456), (4200, 760, 776),
-         (1281, 577, 1160), (1000, 4090, 1096), (9637, 224, 3832)]
+         (1281, 577, 1160), (1000, 4090, 1096), (9637, 224, 3832), (500, 2304, 392), (300, 2328, 776),
+         (1281, 584, 1160), (1000, 4088, 1096)]
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("odt", [BF16, F32])
-@pytest.mark.parametrize("act,resid,ragged", [("none", False, 0), ("gelu_erf", True, 0), ("relu", True, 1)])
+@pytest.mark.parametrize("act,resid,ragged", [("none", False, 0), ("gelu_erf", True, 0), ("relu", True, 1), ("relu", True, 0),
+                                              ("none", True, 8)])
 @pytest.mark.parametrize("M,N,K", TILES)
 def test_every_tile_of_the_persistent_product(gpu, M, N, K, act, resid, ragged, odt):
     _one(M, N - ragged, K, BF16, odt, act, True, resid, seed=33)
