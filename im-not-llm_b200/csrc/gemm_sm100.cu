@@ -439,7 +439,7 @@ __device__ __forceinline__ void epilogue_tile(uint32_t t_row, int row, int n0, i
         tmem_ld_wait();
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-        warp_finish32<TO, false>(linear_args(e), st.buf, v, row0, col, lane, e.aligned != 0);
+        warp_finish32<TO, false, EPI == INL_EPI_LINEAR_F32 && ACT == kLinearPlain ? 8 : 0>(linear_args(e), st.buf, v, row0, col, lane, e.aligned != 0);
       }
     }
   } else {
@@ -507,7 +507,7 @@ __device__ __forceinline__ void epilogue_tile(uint32_t t_row, int row, int n0, i
 // The epilogue of one tile whose sum comes in parts of K (INL_EPI_LINEAR_F32_LONG),
 // for one warp: this thread's row, half of the columns, summed in registers.
 // `taken(acc)` gives accumulator acc back. False: a wait ran out.
-template <int BN, typename Taken>
+template <int BN, bool PLAIN, typename Taken>
 __device__ __forceinline__ bool epilogue_long(uint32_t tmem, uint64_t* tfull, int& acc, uint32_t& acc_phase, int parts,
                                               int row0, int n0, int half, const EpiArgs& e, OutStage& st, int lane,
                                               int* status, Taken taken) {
@@ -538,7 +538,7 @@ __device__ __forceinline__ bool epilogue_long(uint32_t tmem, uint64_t* tfull, in
   for (int c = 0; c < HW; c += 32) {
     const int col = n0 + half * HW + c;
     if (col >= e.N || row0 >= e.M) break;  // warp-uniform
-    warp_finish32<float, false>(linear_args(e), st.buf, sum + c, row0, col, lane, e.aligned != 0);
+    warp_finish32<float, false, PLAIN ? 4 : 0>(linear_args(e), st.buf, sum + c, row0, col, lane, e.aligned != 0);
   }
   return true;
 }
@@ -688,7 +688,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Unit w = unit_of(u, splits, k_blocks);
       const int mb = w.tile / n_tiles, nb = w.tile - (w.tile / n_tiles) * n_tiles;
       if constexpr (LONG) {
-        if (!epilogue_long<BN>(tmem_base + (static_cast<uint32_t>(quad * 32) << 16), tfull, acc, acc_phase,
+        if (!epilogue_long<BN, ACT == kLinearPlain>(tmem_base + (static_cast<uint32_t>(quad * 32) << 16), tfull, acc, acc_phase,
                                (k_blocks + kLongBlocks - 1) / kLongBlocks, mb * kBM + quad * 32, nb * BN, half, e, st,
                                lane, status, [&](int a) {
                                  if (lane == 0) mbar_arrive(&tempty[a]);
@@ -905,7 +905,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Unit w = unit_of(u, splits, k_blocks);
       const int mb = w.tile / n_tiles, nb = w.tile - (w.tile / n_tiles) * n_tiles;
       if constexpr (LONG) {
-        if (!epilogue_long<C::BN>(tmem_base + (static_cast<uint32_t>(quad * 32) << 16), tfull, acc, acc_phase,
+        if (!epilogue_long<C::BN, ACT == kLinearPlain>(tmem_base + (static_cast<uint32_t>(quad * 32) << 16), tfull, acc, acc_phase,
                                   (k_blocks + kLongBlocks - 1) / kLongBlocks,
                                   mb * 2 * kBM + static_cast<int>(rank) * kBM + quad * 32, nb * C::BN, half, e, st,
                                   lane, status, [&](int a) {
@@ -1194,29 +1194,30 @@ int gemm_bf16_tn(const GemmArgs& g, cudaStream_t stream) {
 // Columns of the tile (256: a 256 x 256 tile of a CTA pair; 192, 128, 64: 128 rows
 // of one CTA) that finishes a linear layer first: the tiles' waves over the SMs
 // times the slower of a tile's products and its epilogue, and once the faster of
-// the two. us of a K block and of an epilogue, and per 64 columns of a residual,
-// fitted to 306 random sizes (256 to 131072 rows) x 4 tiles; over those the
-// choice is 0.4% slower than the best tile in the mean, 17% at most. Measured
-// (us), 256 / 192 / 128 / 64, bf16 with gelu: 4253 x 768 x 768 13.7 / 10.7 / 13.5
-// / 15.6; 4253 x 2304 x 768 27 / 21 / 27 / 39; 2048 x 1024 x 1024 14.4 / 11.9 /
-// 10.3 / 13.6; 8192 x 1024 x 2048 33 / 39 / 45 / 69; bf16 to f32: 4253 x 2304 x
-// 768 33 / 23 / 26 / 39; 16384 x 768 x 768 36 / 29 / 30 / 47.
-static int linear_tile(int M, int N, int K, int kind, bool resid) {
+// the two. us of a K block, of an epilogue, and of a residual per 64 columns,
+// fitted to three quarters of 3006 random sizes (256 to 131072 rows) x 4 tiles;
+// over the rest the choice is 0.6% slower than the best tile in the mean and 16%
+// at most. Measured (us), 256 / 192 / 128 / 64, bf16 with gelu: 4253 x 768 x 768
+// 13.7 / 10.7 / 13.5 / 15.6; 4253 x 2304 x 768 27 / 21 / 27 / 39; 2048 x 1024 x
+// 1024 14.4 / 11.9 / 10.3 / 13.6; 8192 x 1024 x 2048 33 / 39 / 45 / 69.
+static int linear_tile(int M, int N, int K, bool out_bf16, bool plain, bool parts, bool resid) {
   constexpr int cols[4] = {256, 192, 128, 64};
-  constexpr float block[4] = {0.40f, 0.35f, 0.32f, 0.30f};
-  constexpr float epilogue[4][4] = {{4.7f, 3.1f, 2.4f, 1.9f},    // bf16, no activation or relu
-                                    {5.7f, 4.1f, 2.9f, 1.6f},    // bf16, another activation
-                                    {0.0f, 4.0f, 3.1f, 1.6f},    // f32, K in one part
-                                    {14.9f, 6.6f, 4.3f, 3.3f}};  // f32, K in parts
+  constexpr float block[4] = {0.40f, 0.36f, 0.36f, 0.30f};
+  constexpr float never = 1e9f;
+  constexpr float epilogue[3][2][4] = {
+      {{6.1f, 4.1f, 3.0f, 1.6f}, {4.8f, 2.6f, 2.0f, 1.1f}},      // bf16; the second without special functions
+      {{never, 4.9f, 3.3f, 1.9f}, {never, 4.3f, 4.2f, 3.5f}},    // f32, K in one part
+      {{16.1f, 11.0f, 7.3f, 7.4f}, {17.0f, 5.1f, 2.2f, 2.9f}}};  // f32, K in parts
+  const float* epi = epilogue[out_bf16 ? 0 : parts ? 2 : 1][plain];
   const long long sms = num_sms();
   const float k_blocks = static_cast<float>((K - 1) / kBK + 1);
   int best = 0;
   float least = 0.f;
-  for (int i = kind == 2 ? 1 : 0; i < 4; ++i) {  // there the pair's tile is never the first
+  for (int i = 0; i < 4; ++i) {
     const long long rows = i == 0 ? 2 * kBM : kBM, at_once = i == 0 ? sms / 2 : sms;
     const long long tiles = ((M + rows - 1) / rows) * ((N + cols[i] - 1ll) / cols[i]);
     const float products = block[i] * k_blocks;
-    const float out = epilogue[kind][i] + (resid ? (kind < 2 ? 0.6f : 1.0f) * static_cast<float>(cols[i] / 64) : 0.f);
+    const float out = epi[i] + (resid ? (out_bf16 ? 0.4f : 3.6f) * static_cast<float>(cols[i] / 64) : 0.f);
     const float time = static_cast<float>((tiles + at_once - 1) / at_once) * std::max(products, out) + std::min(products, out);
     if (best == 0 || time < least) best = cols[i], least = time;
   }
@@ -1250,7 +1251,7 @@ int gemm_bf16_linear(const GemmArgs& g, bool out_bf16, cudaStream_t stream) {
   // result shows. Past 512, such a sum is moved out every 512 of K and added in
   // registers, rounded to nearest (5e-7 at any K).
   const bool parts = !out_bf16 && g.K > kLongBlocks * kBK;
-  const int bn = linear_tile(g.M, g.N, g.K, out_bf16 ? (linear_plain(g.act) ? 0 : 1) : (parts ? 3 : 2), g.resid != nullptr);
+  const int bn = linear_tile(g.M, g.N, g.K, out_bf16, linear_plain(g.act), parts, g.resid != nullptr);
   CUtensorMap ta, tb, to;
   if (!make_kmajor_map(&ta, g.A, g.M, g.K, lda, kBM)) return -2;
   if (!make_kmajor_map(&tb, g.W, g.N, g.K, ldw, bn == 256 ? 128 : bn)) return -2;
@@ -1258,15 +1259,14 @@ int gemm_bf16_linear(const GemmArgs& g, bool out_bf16, cudaStream_t stream) {
   if (out_bf16 && e.aligned &&
       !make_tma_2d_bf16_swizzled(&to, g.out, g.M, g.N, g.M == 1 ? g.N : g.ldo, 32, 32, 64))
     return -2;
-  cudaError_t err;
-  if (out_bf16 && linear_plain(g.act))
-    err = launch_linear<INL_EPI_LINEAR_BF16, kLinearPlain>(bn, ta, tb, to, g.M, g.N, g.K, e, g.status, stream);
-  else if (out_bf16)
-    err = launch_linear<INL_EPI_LINEAR_BF16, kLinearAny>(bn, ta, tb, to, g.M, g.N, g.K, e, g.status, stream);
-  else if (parts)
-    err = launch_linear<INL_EPI_LINEAR_F32_LONG, kLinearAny>(bn, ta, tb, to, g.M, g.N, g.K, e, g.status, stream);
-  else
-    err = launch_linear<INL_EPI_LINEAR_F32, kLinearAny>(bn, ta, tb, to, g.M, g.N, g.K, e, g.status, stream);
+  auto launch = [&](auto act) {
+    constexpr int ACT = decltype(act)::value;
+    return out_bf16 ? launch_linear<INL_EPI_LINEAR_BF16, ACT>(bn, ta, tb, to, g.M, g.N, g.K, e, g.status, stream)
+           : parts  ? launch_linear<INL_EPI_LINEAR_F32_LONG, ACT>(bn, ta, tb, to, g.M, g.N, g.K, e, g.status, stream)
+                    : launch_linear<INL_EPI_LINEAR_F32, ACT>(bn, ta, tb, to, g.M, g.N, g.K, e, g.status, stream);
+  };
+  const cudaError_t err = linear_plain(g.act) ? launch(std::integral_constant<int, kLinearPlain>())
+                                              : launch(std::integral_constant<int, kLinearAny>());
   return err == cudaSuccess ? 0 : -3;
 }
 
