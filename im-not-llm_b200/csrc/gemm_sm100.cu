@@ -439,7 +439,8 @@ __device__ __forceinline__ void epilogue_tile(uint32_t t_row, int row, int n0, i
         tmem_ld_wait();
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-        warp_finish32<TO, false, EPI == INL_EPI_LINEAR_F32 && ACT == kLinearPlain ? 8 : 0>(linear_args(e), st.buf, v, row0, col, lane, e.aligned != 0);
+        constexpr int ahead_rows = EPI == INL_EPI_LINEAR_F32 && ACT == kLinearPlain ? 8 : 0;
+        warp_finish32<TO, false, ahead_rows>(linear_args(e), st.buf, v, row0, col, lane, e.aligned != 0);
       }
     }
   } else {
@@ -688,11 +689,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Unit w = unit_of(u, splits, k_blocks);
       const int mb = w.tile / n_tiles, nb = w.tile - (w.tile / n_tiles) * n_tiles;
       if constexpr (LONG) {
-        if (!epilogue_long<BN, ACT == kLinearPlain>(tmem_base + (static_cast<uint32_t>(quad * 32) << 16), tfull, acc, acc_phase,
-                               (k_blocks + kLongBlocks - 1) / kLongBlocks, mb * kBM + quad * 32, nb * BN, half, e, st,
-                               lane, status, [&](int a) {
-                                 if (lane == 0) mbar_arrive(&tempty[a]);
-                               }))
+        if (!epilogue_long<BN, ACT == kLinearPlain>(
+                tmem_base + (static_cast<uint32_t>(quad * 32) << 16), tfull, acc, acc_phase,
+                (k_blocks + kLongBlocks - 1) / kLongBlocks, mb * kBM + quad * 32, nb * BN, half, e, st, lane, status,
+                [&](int a) {
+                  if (lane == 0) mbar_arrive(&tempty[a]);
+                }))
           break;
         continue;
       }
@@ -905,13 +907,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Unit w = unit_of(u, splits, k_blocks);
       const int mb = w.tile / n_tiles, nb = w.tile - (w.tile / n_tiles) * n_tiles;
       if constexpr (LONG) {
-        if (!epilogue_long<C::BN, ACT == kLinearPlain>(tmem_base + (static_cast<uint32_t>(quad * 32) << 16), tfull, acc, acc_phase,
-                                  (k_blocks + kLongBlocks - 1) / kLongBlocks,
-                                  mb * 2 * kBM + static_cast<int>(rank) * kBM + quad * 32, nb * C::BN, half, e, st,
-                                  lane, status, [&](int a) {
-                                    if (lane == 0)
-                                      mbar_arrive_cluster(tempty_lead0 + static_cast<uint32_t>(a * sizeof(uint64_t)));
-                                  }))
+        if (!epilogue_long<C::BN, ACT == kLinearPlain>(
+                tmem_base + (static_cast<uint32_t>(quad * 32) << 16), tfull, acc, acc_phase,
+                (k_blocks + kLongBlocks - 1) / kLongBlocks, mb * 2 * kBM + static_cast<int>(rank) * kBM + quad * 32,
+                nb * C::BN, half, e, st, lane, status, [&](int a) {
+                  if (lane == 0) mbar_arrive_cluster(tempty_lead0 + static_cast<uint32_t>(a * sizeof(uint64_t)));
+                }))
           break;
         continue;
       }
@@ -1218,7 +1219,8 @@ static int linear_tile(int M, int N, int K, bool out_bf16, bool plain, bool part
     const long long tiles = ((M + rows - 1) / rows) * ((N + cols[i] - 1ll) / cols[i]);
     const float products = block[i] * k_blocks;
     const float out = epi[i] + (resid ? (out_bf16 ? 0.4f : 3.6f) * static_cast<float>(cols[i] / 64) : 0.f);
-    const float time = static_cast<float>((tiles + at_once - 1) / at_once) * std::max(products, out) + std::min(products, out);
+    const float waves = static_cast<float>((tiles + at_once - 1) / at_once);
+    const float time = waves * std::max(products, out) + std::min(products, out);
     if (best == 0 || time < least) best = cols[i], least = time;
   }
   return best;

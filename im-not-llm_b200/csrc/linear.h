@@ -262,7 +262,10 @@ __device__ __forceinline__ void warp_finish32(const LinearArgs& g, uint8_t* buf,
     if (wide && n + 32 <= g.N) {
       const int q = lane & 7, r = lane >> 3, col = n + 4 * q;
       float4 t[PLAIN], d[PLAIN], b = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (g.bias) b = make_float4(__ldg(g.bias + col), __ldg(g.bias + col + 1), __ldg(g.bias + col + 2), __ldg(g.bias + col + 3));
+      if (g.bias) {
+        const float* p = g.bias + col;
+        b = make_float4(__ldg(p), __ldg(p + 1), __ldg(p + 2), __ldg(p + 3));
+      }
       const float* res = static_cast<const float*>(g.resid) + (m + r) * g.ldr + col;
       float* out = static_cast<float*>(g.out) + (m + r) * g.ldo + col;
       auto ahead = [&](int r0) {
