@@ -332,3 +332,11 @@ def test_memory_the_device_cannot_reach_is_refused(gpu):
     n.check(_call(n, torch, pinned, torch.ones(2, 8, device="cuda"), F32, F32, "none", None, None, o), "linear")
     torch.cuda.synchronize()
     assert (o == 8).all()
+
+
+# rows and columns that end inside a warp's 32 x 32 piece of the persistent product's tiles, several pieces to a warp
+@pytest.mark.gpu
+@pytest.mark.parametrize("odt", [BF16, F32])
+@pytest.mark.parametrize("M,N,K", [(1937, 1501, 136), (4129, 763, 72), (1503, 2271, 584), (2079, 1025, 648)])
+def test_pieces_that_end_inside_a_warp(gpu, M, N, K, odt):
+    _one(M, N, K, BF16, odt, "silu", True, True, pad=(-K % 8, -K % 8, 1, 3), seed=41)
