@@ -172,6 +172,7 @@ int gemm_f32_tn(const GemmF32Args& g, cudaStream_t s) {
     case INL_EPI_RESID_BF16: gemm_f32_kernel<INL_EPI_RESID_BF16, 0><<<grid, 256, 0, s>>>(g); break;
     case INL_EPI_GATED_BF16:
       if (g.gate_block != 64 || (g.N % 128) != 0) return -1;
+      if (g.act < INL_ACT_SILU || g.act > INL_ACT_GELU_TANH) return -1;
       switch (g.act) {
         case INL_ACT_SILU: gemm_f32_kernel<INL_EPI_GATED_BF16, INL_ACT_SILU><<<grid, 256, 0, s>>>(g); break;
         case INL_ACT_GELU_ERF: gemm_f32_kernel<INL_EPI_GATED_BF16, INL_ACT_GELU_ERF><<<grid, 256, 0, s>>>(g); break;

@@ -1104,6 +1104,7 @@ int gemm_bf16_tn(const GemmArgs& g, cudaStream_t stream) {
     return -1;
   int bn = (g.N <= 128 || (g.N % 256) != 0) ? 128 : 256;
   if (g.epi == INL_EPI_GATED_BF16 || g.epi == INL_EPI_GATED_F32) {
+    if (g.act < INL_ACT_SILU || g.act > INL_ACT_GELU_TANH) return -1;
     // Gate/up interleaved in blocks of bn/2 rows; the caller picks the block.
     bn = g.gate_block * 2;
     if ((bn != 128 && bn != 256) || (g.N % bn) != 0) return -1;

@@ -30,7 +30,7 @@ extern "C" {
 #define INL_ACT_SILU_ 0
 #define INL_ACT_GELU_ERF_ 1
 #define INL_ACT_GELU_TANH_ 2
-/* inl_cuda_linear only: */
+/* inl_cuda_linear only; the gated epilogues refuse them (INL_ERR_INVALID_INPUT): */
 #define INL_ACT_NONE_ 3
 #define INL_ACT_RELU_ 4
 #define INL_ACT_TANH_ 5

@@ -146,6 +146,20 @@ def test_refusals_need_no_gpu():
     assert call(N=0, w=None, out=None) == 0
 
 
+@pytest.mark.parametrize("act", [-1, ACTS["none"], ACTS["relu"], ACTS["tanh"], 6])
+def test_gated_products_refuse_the_linear_layers_activations(act):
+    """They know silu and the two gelus; another code is not read as one of these."""
+    n = _n()
+    f = n.lib()
+    for epi, block in ((2, 64), (2, 128), (7, 128)):  # INL_GEMM_EPI_GATED, _GATED_F32
+        args = n.GemmEx()
+        args.A, args.W, args.out, args.lda, args.ldw, args.ldo = 256, 256, 256, 64, 64, 128
+        args.M, args.N, args.K, args.epi, args.act, args.gate_block = 8, 256, 64, epi, act, block
+        assert f.inl_cuda_gemm_bf16_ex(ctypes.byref(args), None) == INVALID
+        assert f.inl_cuda_gemm_bf16(256, 64, 256, 64, 8, 256, 64, epi, act, block, 256, 128, None, 0, 0, None, None) == INVALID
+    assert f.inl_cuda_gemm_f32(256, 64, 256, 64, 8, 256, 64, 2, act, 256, 128, None, 0, None) == INVALID
+
+
 # ---------------------------------------------------------------- GPU
 SHAPES = [(1, 1, 1), (1, 4096, 1024), (2, 7, 3), (5, 3, 0), (3, 33, 17), (8, 256, 128), (16, 1000, 520),
           (17, 1024, 2048), (33, 130, 72), (64, 64, 64), (65, 96, 4096), (129, 513, 264), (300, 768, 768),
