@@ -354,3 +354,33 @@ def test_memory_the_device_cannot_reach_is_refused(gpu):
 @pytest.mark.parametrize("M,N,K", [(1937, 1501, 136), (4129, 763, 72), (1503, 2271, 584), (2079, 1025, 648)])
 def test_pieces_that_end_inside_a_warp(gpu, M, N, K, odt):
     _one(M, N, K, BF16, odt, "silu", True, True, pad=(-K % 8, -K % 8, 1, 3), seed=41)
+
+
+# Left of zero gelu and silu fall to 1e-14 of their argument; an f32 result keeps its digits there. The pre-activation
+# sum is the bias alone (x is zero), so exact; relative to |y|, by the arithmetic of the formulas in linear.h:
+# erfc's argument is off by 2u, times the slope 2 t^2 + 1 = x^2 + 1, its own error 8u (4 ulp), two products: (2 x^2 + 12) u;
+# exp's argument w is off by 5u |w|, its own error 4u, a sum and a quotient: (5 |w| + 8) u.
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,M,K", [(BF16, 3, 64), (BF16, 130, 1024), (BF16, 700, 64), (BF16, 700, 1024), (F32, 3, 64),
+                                    (F32, 130, 1024), (F32, 1500, 64), (BF16, 9, 61), (F32, 150, 61)])
+@pytest.mark.parametrize("act", ["silu", "gelu_erf", "gelu_tanh"])
+def test_f32_activations_keep_their_digits_on_the_tail(gpu, act, dt, M, K):
+    import math
+
+    import torch
+
+    n = _n()
+    N = 1500
+    x = torch.zeros(M, K, device="cuda", dtype=_dt(torch, dt))
+    w = torch.ones(N, K, device="cuda", dtype=_dt(torch, dt))
+    v = torch.linspace(-8, 3, N, device="cuda")
+    out = torch.empty(M, N, device="cuda")
+    n.check(_call(n, torch, x, w, dt, F32, act, v, None, out), "linear")
+    torch.cuda.synchronize()
+    z = v.double()
+    if act == "gelu_erf":
+        want, tol = 0.5 * z * torch.special.erfc(-z / math.sqrt(2)), (2 * z * z + 12) * U
+    else:
+        arg = z if act == "silu" else 2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)
+        want, tol = z / (1 + torch.exp(-arg)), (5 * arg.abs() + 8) * U
+    assert ((out.double() - want).abs() <= tol * want.abs() + 1e-37).all(), ((out.double() - want).abs() / want.abs()).max().item()
