@@ -183,21 +183,54 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
                : "r"(addr));
   return v;
 }
-// A plain f32 sum, ended by the first NaN.
+// Counted up while a NaN is computed again, for the waits that this makes long
+// (wait_alive). A static shared variable: its address takes no register.
+__device__ __forceinline__ unsigned* redo_beat() {
+  __shared__ unsigned beat;
+  return &beat;
+}
+__device__ __forceinline__ unsigned redo_beats() { return *reinterpret_cast<const volatile unsigned*>(redo_beat()); }
+
+// A plain f32 sum, ended by the first NaN. BEAT: others wait for it (redo_beat).
+template <bool BEAT>
 __device__ __forceinline__ float plain_dot(const LinearArgs& g, long long m, long long n) {
   const float* x = static_cast<const float*>(g.x) + m * g.ldx;
   const float* w = static_cast<const float*>(g.w) + n * g.ldw;
   float s = 0.f;
-  for (int k = 0; k < g.K && !isnan(s); ++k) s = fmaf(x[k], w[k], s);
+  for (int k = 0; k < g.K && !isnan(s); ++k) {
+    s = fmaf(x[k], w[k], s);
+    if (BEAT && (k & 0xfff) == 0) atomicAdd(redo_beat(), 1u);
+  }
   return s;
 }
 
 // The NaNs among the sums v of row m, columns n .. n + 3, again.
+template <bool BEAT>
 __device__ __forceinline__ void redo4(const LinearArgs& g, float4& v, long long m, int n) {
-  if (isnan(v.x)) v.x = plain_dot(g, m, n);
-  if (isnan(v.y) && n + 1 < g.N) v.y = plain_dot(g, m, n + 1);
-  if (isnan(v.z) && n + 2 < g.N) v.z = plain_dot(g, m, n + 2);
-  if (isnan(v.w) && n + 3 < g.N) v.w = plain_dot(g, m, n + 3);
+  if (isnan(v.x)) v.x = plain_dot<BEAT>(g, m, n);
+  if (isnan(v.y) && n + 1 < g.N) v.y = plain_dot<BEAT>(g, m, n + 1);
+  if (isnan(v.z) && n + 2 < g.N) v.z = plain_dot<BEAT>(g, m, n + 2);
+  if (isnan(v.w) && n + 3 < g.N) v.w = plain_dot<BEAT>(g, m, n + 3);
+}
+
+// A wait whose limit starts anew whenever redo_beat has moved: what it waits for
+// may be behind a lane that computes NaNs again, for as long as K is.
+__device__ __forceinline__ bool wait_alive(uint64_t* bar, uint32_t parity, int* status, int code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  unsigned seen = redo_beats();
+  uint64_t t0 = globaltimer_ns();
+  while (true) {
+    if (mbar_try_wait_sleep(bar, parity, 100000u)) return true;
+    if (globaltimer_ns() - t0 > INL_WAIT_TIMEOUT_NS) {
+      const unsigned now = redo_beats();
+      if (now == seen) {
+        if (status) atomicCAS(status, 0, code);
+        return false;
+      }
+      seen = now;
+      t0 = globaltimer_ns();
+    }
+  }
 }
 
 // After a cluster barrier: 256 threads (tid) of each of the S CTAs sum their
@@ -235,7 +268,7 @@ __device__ __forceinline__ void cluster_finish(const LinearArgs& g, uint8_t* par
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (i >= count || !isnan(v[i].x + v[i].y + v[i].z + v[i].w)) continue;
-        redo4(g, v[i], m0 + r0 + i * S * STEP, n);
+        redo4<false>(g, v[i], m0 + r0 + i * S * STEP, n);
       }
     }
 #pragma unroll
@@ -319,7 +352,7 @@ __device__ __forceinline__ void warp_finish32(const LinearArgs& g, uint8_t* buf,
       for (int i = 0; i < 4; ++i) {
         const int rr = r + 4 * i;
         t[i] = *reinterpret_cast<const float4*>(buf + rr * 128 + ((q ^ (rr & 7)) << 4));
-        if (REDO && isnan(t[i].x + t[i].y + t[i].z + t[i].w) && i < count) redo4(g, t[i], m + rr, col);
+        if (REDO && isnan(t[i].x + t[i].y + t[i].z + t[i].w) && i < count) redo4<true>(g, t[i], m + rr, col);
         t[i].x += b[0], t[i].y += b[1], t[i].z += b[2], t[i].w += b[3];
       }
       linear_finish_rows<TO, 4>(g, t, m + r, 4, count, col, wide);

@@ -14,7 +14,10 @@
 // A CTA walks over 128 x 128 tiles, or a cluster of S CTAs shares out the K of
 // one, as in linear_cluster_kernel. A sum that comes out NaN is computed again as
 // a plain f32 sum: the split turns an infinite (or rounding to infinity) operand
-// into inf - inf, and a row that holds one must still give what f32 gives.
+// into inf - inf, and a row that holds one must still give what f32 gives. One lane
+// computes it, 0.14 us per element of K: 1024 x 1024 x 1024 with an infinity in every
+// row 4.7 ms, 1024 x 4736 x 320000 5 s, which is why waits behind it end only when
+// it stands still (wait_alive).
 //
 // 1024 x 4096 x 1024: 56 us = 154 TFLOP/s of f32, off by 3.5e-7 (an f32 library
 // product: 162 us, off by 5.7e-7); 8192 x 4096 x 4096: 1.35 ms = 203 TFLOP/s,
@@ -136,6 +139,7 @@ __global__ void __launch_bounds__(threads_of(TMA), 1)
       mbar_init(&xfree[a], 1);
     }
     mbar_init(sempty, 8);
+    if (TMA) *redo_beat() = 0;
     fence_barrier_init();
     if (TMA) {
       tma_prefetch_desc(&tmA);
@@ -152,6 +156,12 @@ __global__ void __launch_bounds__(threads_of(TMA), 1)
   const uint32_t tmem = *tmem_holder;
   pdl_wait();
 
+  // CTAs that walk over tiles compute NaNs again under the next tile's products: every wait may be behind that
+  auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+    return TMA ? wait_alive(bar, parity, status, code) : mbar_wait(bar, parity, status, code);
+  };
+  auto wait_warp = [&](uint64_t* bar, uint32_t parity, int code) { return __all_sync(0xffffffffu, wait(bar, parity, code)); };
+
   if (warp == 0) {
     if (TMA && lane == 0) {
       Ring in;
@@ -160,7 +170,7 @@ __global__ void __launch_bounds__(threads_of(TMA), 1)
       for (int tile = first; tile < end && ok; tile += stride) {
         const int m0 = tile / n_tiles * kBM, n0 = tile % n_tiles * kBN;
         for (int i = 0; i < nkb; ++i, in.next(kStages)) {
-          if (!(ok = mbar_wait(&empty[in.slot], in.phase ^ 1, status, INL_DEV_TIMEOUT_PRODUCER))) break;
+          if (!(ok = wait(&empty[in.slot], in.phase ^ 1, INL_DEV_TIMEOUT_PRODUCER))) break;
           uint8_t* base = smem + in.slot * kStageBytes;
           mbar_expect_tx(&full[in.slot], 2 * kTile);
           tma_load_2d(base, &tmA, &full[in.slot], (kb0 + i) * kBK, m0);
@@ -172,7 +182,7 @@ __global__ void __launch_bounds__(threads_of(TMA), 1)
       for (int f = issued; f > 0; --f) {
         const int back = in.slot - f;  // slots before in.slot are in this phase, the others in the one before
         const int slot = back < 0 ? back + kStages : back;
-        if (!mbar_wait(&full[slot], back < 0 ? in.phase ^ 1 : in.phase, status, INL_DEV_TIMEOUT_DRAIN)) break;
+        if (!wait(&full[slot], back < 0 ? in.phase ^ 1 : in.phase, INL_DEV_TIMEOUT_DRAIN)) break;
       }
     }
   } else if (warp == 1) {
@@ -183,12 +193,12 @@ __global__ void __launch_bounds__(threads_of(TMA), 1)
       uint32_t tile_phase = 0;
       bool ok = true;
       for (int tile = first; tile < end && ok; tile += stride, tile_phase ^= 1) {
-        if (!(ok = mbar_wait(sempty, tile_phase ^ 1, status, INL_DEV_TIMEOUT_MMA))) break;
+        if (!(ok = wait(sempty, tile_phase ^ 1, INL_DEV_TIMEOUT_MMA))) break;
         for (int i = 0; i < nkb; ++i, out.next(kStages), x.next(2)) {
           if (i % kChunk == 0 &&
-              !(ok = mbar_wait(&tempty[acc.slot], acc.phase ^ 1, status, INL_DEV_TIMEOUT_MMA)))
+              !(ok = wait(&tempty[acc.slot], acc.phase ^ 1, INL_DEV_TIMEOUT_MMA)))
             break;
-          if (!(ok = mbar_wait(&split[out.slot], out.phase, status, INL_DEV_TIMEOUT_MMA))) break;
+          if (!(ok = wait(&split[out.slot], out.phase, INL_DEV_TIMEOUT_MMA))) break;
           tc_fence_after();
           // a stage: x, w hi, w lo (TMA); x hi, w hi, x lo, w lo
           const uint64_t st = sw128_kmajor_desc(smem_u32(smem + out.slot * kStageBytes)), wh = st + (kTile >> 4);
@@ -232,7 +242,7 @@ __global__ void __launch_bounds__(threads_of(TMA), 1)
 #pragma unroll
       for (int j = 0; j < R; ++j) sum[j] = 0.f;
       for (int c = 0; c < chunks; ++c, acc.next(2)) {
-        if (!(ok = mbar_wait_warp(&tfull[acc.slot], acc.phase, status, INL_DEV_TIMEOUT_EPILOGUE))) break;
+        if (!(ok = wait_warp(&tfull[acc.slot], acc.phase, INL_DEV_TIMEOUT_EPILOGUE))) break;
         tc_fence_after();
 #pragma unroll
         for (int j = 0; j < 64; j += 16) {
@@ -296,7 +306,7 @@ __global__ void __launch_bounds__(threads_of(TMA), 1)
     load_rows(
         rows, kb0, nkb, kBK,
         [&](int i) {
-          return mbar_wait_warp(&empty[i % kStages], ((i / kStages) & 1) ^ 1, status, INL_DEV_TIMEOUT_PRODUCER);
+          return wait_warp(&empty[i % kStages], ((i / kStages) & 1) ^ 1, INL_DEV_TIMEOUT_PRODUCER);
         },
         [&](int i, int j, uint32_t word) {
           const float v = __uint_as_float(word), h = tf32_of(v);
@@ -318,8 +328,8 @@ __global__ void __launch_bounds__(threads_of(TMA), 1)
     for (int tile = first; tile < end && ok; tile += stride) {
       for (int i = 0; i < nkb; ++i, in.next(kStages), x.next(2)) {
         const bool of_x = warp < 10 + kSplitX;
-        if (of_x && !(ok = mbar_wait_warp(&xfree[x.slot], x.phase ^ 1, status, INL_DEV_TIMEOUT_PRODUCER))) break;
-        if (!(ok = mbar_wait_warp(&full[in.slot], in.phase, status, INL_DEV_TIMEOUT_PRODUCER))) break;
+        if (of_x && !(ok = wait_warp(&xfree[x.slot], x.phase ^ 1, INL_DEV_TIMEOUT_PRODUCER))) break;
+        if (!(ok = wait_warp(&full[in.slot], in.phase, INL_DEV_TIMEOUT_PRODUCER))) break;
         uint8_t* const at = smem + in.slot * kStageBytes;
         if (of_x) {
           // x: thread = row (lane quadrant warp % 4), from shared memory to TMEM

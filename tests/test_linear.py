@@ -384,3 +384,65 @@ def test_f32_activations_keep_their_digits_on_the_tail(gpu, act, dt, M, K):
         arg = z if act == "silu" else 2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)
         want, tol = z / (1 + torch.exp(-arg)), (5 * arg.abs() + 8) * U
     assert ((out.double() - want).abs() <= tol * want.abs() + 1e-37).all(), ((out.double() - want).abs() / want.abs()).max().item()
+
+
+# f32 operands that a split into tf32 halves cannot carry: infinities, NaNs and values that round to infinity there, in every
+# row and column or in some, through every kernel (few rows; K shared by clusters; tiles walked over; rows of odd strides)
+@pytest.mark.gpu
+@pytest.mark.parametrize("odd", [0, 1])
+@pytest.mark.parametrize("M,N,K", [(5, 300, 136), (40, 264, 1100), (140, 264, 520), (1300, 1000, 1100), (2500, 1801, 136)])
+@pytest.mark.parametrize("where", ["every row of x", "every row of w", "some of each", "huge"])
+def test_f32_values_that_do_not_split(gpu, where, M, N, K, odd):
+    import torch
+
+    n = _n()
+    inf, nan = float("inf"), float("nan")
+    x, _ = _rows(torch, M, K, odd, F32, 3)
+    w, _ = _rows(torch, N, K, 3 * odd, F32, 4, 0.01)
+    r, _ = _rows(torch, M, N, odd, F32, 5)
+    if where == "every row of x":
+        x[:, 5] = inf
+    elif where == "every row of w":
+        w[:, K - 1] = -inf
+    elif where == "some of each":
+        x[::7, 1], x[3::11, K // 2], x[::7, K - 2], w[::5, 3], w[1, :] = inf, -inf, inf, inf, 0
+        x[2, 2], w[4, 2], x[1, 3] = nan, nan, 0
+    else:
+        x[:, 7], w[::3, 9], x[::2, 9], w[:, 7] = 3.4028e38, -3.4028e38, 1e-3, 0.3
+    out = torch.zeros(M, N + odd, device="cuda")[:, :N]
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    n.check(_call(n, torch, x, w, F32, F32, "none", None, r, out, status=st), "linear")
+    torch.cuda.synchronize()
+    z, S, y = _want(torch, x, w, None, "none", r)
+    assert st.item() == 0
+    # a sum whose products pass f32's range in sum may overflow on the way, or not, by their order: not compared
+    sure = ~torch.isfinite(S) | (S <= torch.finfo(torch.float32).max)
+    assert torch.equal(torch.isnan(out)[sure], torch.isnan(y)[sure])
+    far = torch.isinf(y)
+    assert torch.equal(torch.isinf(out)[sure], far[sure]) and torch.equal(out[far].double(), y[far])
+    ok = torch.isfinite(y) & sure
+    tol = 2 * U * (K + 2) * S[ok] + 4 * U * (y[ok].abs() + r.double()[ok].abs())
+    assert ((out.double()[ok] - y[ok]).abs() <= tol + 1e-37).all()
+
+
+@pytest.mark.gpu
+def test_many_long_sums_computed_again_outlast_no_wait(gpu):
+    """Every sum of a tile is computed again, for longer than a wait's limit (2 s), while the next tile's products wait for
+    its place: that is work, not a wait that ran out."""
+    import torch
+
+    n = _n()
+    M, N, K = 1024, 4736, 320000
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs 16 GB")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.rand(M, K, generator=g, device="cuda")
+    w = torch.rand(N, K, generator=g, device="cuda")
+    w[::2] *= -1
+    x[:, 5] = float("inf")
+    out = torch.zeros(M, N, device="cuda")
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    n.check(_call(n, torch, x, w, F32, F32, "none", None, None, out, status=st), "linear")
+    torch.cuda.synchronize()
+    assert st.item() == 0
+    assert torch.equal(out, torch.where(w[:, 5] > 0, float("inf"), -float("inf")).expand(M, N))
