@@ -991,8 +991,7 @@ cudaError_t launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUte
   int grid = num_sms();
   if (max_ctas > 0 && max_ctas < grid) grid = max_ctas;
   if (tiles < grid) grid = tiles;
-  cudaError_t err = launch_pdl(kern, dim3(grid), dim3(kThreads), C::SMEM_BYTES, stream, ta, tb, to, M, N, K, e, status);
-  return err != cudaSuccess ? err : cudaGetLastError();
+  return launch_pdl(kern, dim3(grid), dim3(kThreads), C::SMEM_BYTES, stream, ta, tb, to, M, N, K, e, status);
 }
 
 template <int EPI, int ACT>
@@ -1007,9 +1006,7 @@ cudaError_t launch_gemm_pair(const CUtensorMap& ta, const CUtensorMap& tb, const
   int pairs = num_sms() / 2;
   if (max_ctas > 0 && max_ctas / 2 < pairs) pairs = max_ctas / 2 > 0 ? max_ctas / 2 : 1;
   if (tiles < pairs) pairs = tiles;
-  cudaError_t err =
-      launch_pdl(kern, dim3(2 * pairs), dim3(kThreads), C::SMEM_BYTES, stream, ta, tb, to, M, N, K, e, status);
-  return err != cudaSuccess ? err : cudaGetLastError();
+  return launch_pdl(kern, dim3(2 * pairs), dim3(kThreads), C::SMEM_BYTES, stream, ta, tb, to, M, N, K, e, status);
 }
 
 template <int EPI>

@@ -54,11 +54,11 @@ inline int check_reachable(const char* what, std::initializer_list<HookPtr> ptrs
   return INL_OK;
 }
 
-// Status of a launch: the error is read (and cleared) here.
+// The status e that a launch returned. An error that an earlier call left on
+// this thread is not taken for the launch's, and stays for its owner to read.
 inline int launched(const char* what, cudaError_t e) {
-  const cudaError_t last = cudaGetLastError();
-  if (e == cudaSuccess) e = last;
   if (e == cudaSuccess) return INL_OK;
+  (void)cudaGetLastError();  // the launch's own
   return record_error(INL_ERR_INFERENCE, std::string(what) + " launch failed: " + cudaGetErrorString(e));
 }
 

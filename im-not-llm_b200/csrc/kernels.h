@@ -121,6 +121,19 @@ inline cudaError_t set_smem_limit_once(Kernel kern, int bytes, std::atomic<unsig
   return err;
 }
 
+// Launch whose status is this launch's own (the <<<>>> form leaves it to
+// cudaGetLastError, which may hold an earlier call's error and clears it).
+template <typename... Params, typename... Args>
+inline cudaError_t launch_plain(void (*kern)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
+                                Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
 // Launch with programmatic stream serialization: the kernel may start while
 // its predecessor in the stream finishes, and must call pdl_wait() before it
 // reads anything the predecessor wrote.

@@ -85,8 +85,7 @@ template <typename TX, typename TO, int MT, int V>
 cudaError_t launch_rows(const LinearArgs& g, cudaStream_t s) {
   constexpr int R = 4;
   const dim3 grid((g.N + R - 1) / R, std::min((g.M + MT - 1) / MT, 65535));
-  linear_rows_kernel<TX, TO, MT, R, V><<<grid, 256, 0, s>>>(g);
-  return cudaGetLastError();
+  return launch_plain(linear_rows_kernel<TX, TO, MT, R, V>, grid, dim3(256), 0, s, g);
 }
 
 template <typename TX, typename TO, int V>
@@ -177,7 +176,9 @@ int linear(const LinearArgs& g, int dtype, int out_dtype, int* status, cudaStrea
     if (S > 1) return launched("linear", linear_cluster(g, ob, true, S, status, s));
     const int rc = gemm_bf16_linear(t, ob, s);
     if (rc == 0) return INL_OK;
-    return record_error(INL_ERR_INFERENCE, rc == -3 ? "linear launch failed" : "linear: no TMA map for x, w or out");
+    return record_error(INL_ERR_INFERENCE,
+                        rc == -3 ? std::string("linear launch failed: ") + cudaGetErrorString(cudaGetLastError())
+                                 : std::string("linear: no TMA map for x, w or out"));
   }
   const bool aligned = xb ? gemm_bf16_linear_takes(t) : linear_f32_takes(g);
   // Few rows, where the product is a read of w. Measured (us), linear_rows /

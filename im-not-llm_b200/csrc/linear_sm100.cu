@@ -108,8 +108,8 @@ __global__ void __launch_bounds__(32 * W) linear_skinny_kernel(LinearArgs g) {
 
 template <typename TO, int MT, int NT, int U, int W>
 cudaError_t launch_skinny(const LinearArgs& g, cudaStream_t s) {
-  linear_skinny_kernel<TO, MT, NT, U, W><<<(g.N + 8 * NT - 1) / (8 * NT), 32 * W, W * MT * 16 * (NT * 8 + 1) * 4, s>>>(g);
-  return cudaGetLastError();
+  return launch_plain(linear_skinny_kernel<TO, MT, NT, U, W>, dim3((g.N + 8 * NT - 1) / (8 * NT)), dim3(32 * W),
+                      W * MT * 16 * (NT * 8 + 1) * 4, s, g);
 }
 
 template <typename TO>

@@ -149,8 +149,7 @@ template <typename T, int NORM>
 cudaError_t launch_any(const RotaryArgs& a, cudaStream_t s) {
   const long long items = static_cast<long long>(a.T) * (a.set[0].heads + a.set[1].heads);
   const long long blocks = std::min<long long>((items + 7) / 8, 1 << 20);
-  rotary_any_kernel<T, NORM><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
-  return cudaGetLastError();
+  return launch_plain(rotary_any_kernel<T, NORM>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a);
 }
 
 // E consecutive values in one access.
@@ -389,8 +388,7 @@ cudaError_t launch_vec(const RotaryArgs& a, cudaStream_t s) {
   const size_t smem = (static_cast<size_t>(half) << log_tokens) * 64 + (NORM == kNoNorm ? 0 : 16 * a.d) + 8 * half;
   auto kern = rotary_vec_kernel<T, E, NORM, INTER, KI>;
   const dim3 grid(std::min((tiles - 1) / 8 + 1, sms * 4), runs);
-  kern<<<grid, 256, smem, s>>>(a, log_lanes, log_tokens, run);
-  return cudaGetLastError();
+  return launch_plain(kern, grid, dim3(256), smem, s, a, log_lanes, log_tokens, run);
 }
 
 // Whether heads, pairs and rows come apart into E-vectors, 32 units to a head at most.
