@@ -6,7 +6,10 @@
 // in between: the k order inside a product is free as long as x and w agree, so
 // a lane takes 16 contiguous bytes of its row as the k pairs (0,1 | 8,9) of one
 // m16n8k16 and of the next. A CTA owns 8 NT rows of w, its 8 or 16 warps split K
-// and are summed in shared memory in warp order. A read of w bounds it: one row x
+// and are summed in shared memory in warp order. The tensor core truncates its
+// sums, so each holds 64 to 256 of K and they are added to nearest (in one
+// accumulator all along, sums of one sign were off by 8e-7 at K = 16384, by
+// 3e-4 at 2^20). A read of w bounds it: one row x
 // 4096 x 1024 3.2 us = 2.6 TB/s, of which launch and one trip to memory are 2.
 //
 // linear_cluster_kernel: some hundreds of rows, or few columns. A cluster of S
@@ -57,9 +60,10 @@ __global__ void __launch_bounds__(32 * W) linear_skinny_kernel(LinearArgs g) {
   const int r = lane >> 2, kq = (lane & 3) * 8;
   const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(g.x);
   const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(g.w);
-  float acc[MT][NT][4] = {};
+  float sum[MT][NT][4] = {};
   const uint4 zero = make_uint4(0, 0, 0, 0);
   for (int k0 = warp * 32; k0 < g.K; k0 += W * 32 * U) {
+    float acc[MT][NT][4] = {};
     uint4 wv[U][NT], xv[U][MT][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -88,13 +92,19 @@ __global__ void __launch_bounds__(32 * W) linear_skinny_kernel(LinearArgs g) {
           mma_bf16_16816(acc[i][j], lo.z, hi.z, lo.w, hi.w, wv[u][j].z, wv[u][j].w);
         }
       }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[i][j][e] += acc[i][j][e];
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) red[warp][i * 16 + r + (e >> 1) * 8][j * 8 + (lane & 3) * 2 + (e & 1)] = acc[i][j][e];
+      for (int e = 0; e < 4; ++e) red[warp][i * 16 + r + (e >> 1) * 8][j * 8 + (lane & 3) * 2 + (e & 1)] = sum[i][j][e];
   __syncthreads();
   for (int o = threadIdx.x; o < MT * 16 * NT * 8; o += 32 * W) {
     const int m = o / (NT * 8), c = o % (NT * 8), n = n0 + c;

@@ -499,3 +499,27 @@ def test_an_earlier_calls_error_is_not_taken_for_a_launchs(gpu):
     r = subprocess.run([sys.executable, "-c", STALE], capture_output=True, text=True, timeout=300,
                        cwd=Path(__file__).resolve().parents[1])
     assert r.returncode == 0 and "fine" in r.stdout, r.stdout + r.stderr
+
+
+# Sums of one sign show what an accumulator that truncates loses. A part of c products (512 of K; f32 operands 128) is c / 16
+# (f32: c / 8) instructions' worth of truncated adds, each below 2u of a sum that grows evenly: (c / 16 + 1) u of the part;
+# the parts are added to nearest, sqrt(K / c) u of the whole in the norm. f32 operands: 2^-21 of each, below 20u, beside.
+# Kept in one accumulator the sums are off by 1e-9 K: 74u at 4096, 1100u at 65536 (a warp's share of few rows: 130u).
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [4096, 65536])
+@pytest.mark.parametrize("dt,odd", [(BF16, 0), (BF16, 1), (F32, 0), (F32, 1)])
+@pytest.mark.parametrize("M,N", [(1, 1030), (12, 1100), (14, 5000), (24, 1000), (24, 5000), (50, 1000), (130, 264), (300, 520),
+                                 (1000, 264), (520, 2300), (1300, 1000)])
+def test_long_sums_of_one_sign(gpu, M, N, dt, odd, K):
+    import torch
+
+    n = _n()
+    g = torch.Generator(device="cuda").manual_seed(M + N)
+    x = (torch.rand(M, K + odd, generator=g, device="cuda") + 0.5).to(_dt(torch, dt))[:, :K]
+    w = (torch.rand(N, K + odd, generator=g, device="cuda") + 0.5).to(_dt(torch, dt))[:, :K]
+    out = torch.empty(M, N, device="cuda")
+    n.check(_call(n, torch, x, w, dt, F32, "none", None, None, out), "linear")
+    want = sum(x[:, k:k + 8192].double() @ w[:, k:k + 8192].double().T for k in range(0, K, 8192))
+    rel = ((out.double() - want).norm() / want.norm()).item()
+    limit = (33 + (K / 512) ** 0.5) * U if dt == BF16 else (17 + 20 + (K / 128) ** 0.5) * U
+    assert rel <= limit, (rel / U, limit / U)
