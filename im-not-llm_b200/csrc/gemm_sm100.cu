@@ -35,7 +35,9 @@ constexpr int kBM = 128;
 constexpr int kBK = 64;  // one 128-byte swizzle row of bf16
 constexpr int kEpiWarps = 8;  // two warps per TMEM lane quadrant, each owning half of the tile's columns
 constexpr int kThreads = 64 + 32 * kEpiWarps;
-constexpr int kLongBlocks = 8;  // K blocks between promotions of INL_EPI_LINEAR_F32_LONG
+constexpr int kLongBlocks = 8;  // K blocks between promotions of the sum (epi_long)
+constexpr int kLongBf16 = 32768;  // K past which a bf16 result takes them
+__host__ __device__ constexpr bool epi_long(int epi) { return epi == INL_EPI_LINEAR_F32_LONG || epi == INL_EPI_LINEAR_BF16_LONG; }
 
 template <int BN>
 struct GemmCfg {
@@ -505,10 +507,9 @@ __device__ __forceinline__ void epilogue_tile(uint32_t t_row, int row, int n0, i
   }
 }
 
-// The epilogue of one tile whose sum comes in parts of K (INL_EPI_LINEAR_F32_LONG),
-// for one warp: this thread's row, half of the columns, summed in registers.
+// The epilogue of one tile whose sum comes in parts of K (epi_long), for one warp: this thread's row, half of the columns, summed in registers.
 // `taken(acc)` gives accumulator acc back. False: a wait ran out.
-template <int BN, bool PLAIN, typename Taken>
+template <int BN, int EPI, bool PLAIN, typename Taken>
 __device__ __forceinline__ bool epilogue_long(uint32_t tmem, uint64_t* tfull, int& acc, uint32_t& acc_phase, int parts,
                                               int row0, int n0, int half, const EpiArgs& e, OutStage& st, int lane,
                                               int* status, Taken taken) {
@@ -539,7 +540,9 @@ __device__ __forceinline__ bool epilogue_long(uint32_t tmem, uint64_t* tfull, in
   for (int c = 0; c < HW; c += 32) {
     const int col = n0 + half * HW + c;
     if (col >= e.N || row0 >= e.M) break;  // warp-uniform
-    warp_finish32<float, false, PLAIN ? 4 : 0>(linear_args(e), st.buf, sum + c, row0, col, lane, e.aligned != 0);
+    using TO = std::conditional_t<EPI == INL_EPI_LINEAR_F32_LONG, float, __nv_bfloat16>;
+    constexpr int ahead_rows = EPI == INL_EPI_LINEAR_F32_LONG && PLAIN ? 4 : 0;
+    warp_finish32<TO, false, ahead_rows>(linear_args(e), st.buf, sum + c, row0, col, lane, e.aligned != 0);
   }
   return true;
 }
@@ -569,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int k_blocks = (K + kBK - 1) / kBK;
   const int splits = e.splits > 1 ? e.splits : 1;
   const int num_units = num_tiles * splits;
-  constexpr bool LONG = EPI == INL_EPI_LINEAR_F32_LONG;
+  constexpr bool LONG = epi_long(EPI);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -689,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Unit w = unit_of(u, splits, k_blocks);
       const int mb = w.tile / n_tiles, nb = w.tile - (w.tile / n_tiles) * n_tiles;
       if constexpr (LONG) {
-        if (!epilogue_long<BN, ACT == kLinearPlain>(
+        if (!epilogue_long<BN, EPI, ACT == kLinearPlain>(
                 tmem_base + (static_cast<uint32_t>(quad * 32) << 16), tfull, acc, acc_phase,
                 (k_blocks + kLongBlocks - 1) / kLongBlocks, mb * kBM + quad * 32, nb * BN, half, e, st, lane, status,
                 [&](int a) {
@@ -778,7 +781,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int k_blocks = (K + kBK - 1) / kBK;
   const int splits = e.splits > 1 ? e.splits : 1;
   const int num_units = num_tiles * splits;
-  constexpr bool LONG = EPI == INL_EPI_LINEAR_F32_LONG;
+  constexpr bool LONG = epi_long(EPI);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -907,7 +910,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Unit w = unit_of(u, splits, k_blocks);
       const int mb = w.tile / n_tiles, nb = w.tile - (w.tile / n_tiles) * n_tiles;
       if constexpr (LONG) {
-        if (!epilogue_long<C::BN, ACT == kLinearPlain>(
+        if (!epilogue_long<C::BN, EPI, ACT == kLinearPlain>(
                 tmem_base + (static_cast<uint32_t>(quad * 32) << 16), tfull, acc, acc_phase,
                 (k_blocks + kLongBlocks - 1) / kLongBlocks, mb * 2 * kBM + static_cast<int>(rank) * kBM + quad * 32,
                 nb * C::BN, half, e, st, lane, status, [&](int a) {
@@ -1248,19 +1251,23 @@ int gemm_bf16_linear(const GemmArgs& g, bool out_bf16, cudaStream_t stream) {
   if (out_bf16 && g.N % 8 != 0) e.aligned = 0;
   // The tensor core's f32 accumulator truncates: a sum of K = 1024 products is
   // off by 1e-6 of itself toward zero, one of 4096 by 4.4e-6, which an f32
-  // result shows. Past 512, such a sum is moved out every 512 of K and added in
-  // registers, rounded to nearest (5e-7 at any K).
-  const bool parts = !out_bf16 && g.K > kLongBlocks * kBK;
-  const int bn = linear_tile(g.M, g.N, g.K, out_bf16, linear_plain(g.act), parts, g.resid != nullptr);
+  // result shows past 512 and a bf16 one (half a step: 2e-3 of the value) past
+  // some ten thousand. Such a sum is moved out every 512 of K and added in
+  // registers, rounded to nearest: products of one sign 2.4e-7 off at K = 1024, 2.8e-7
+  // at 65536. It also keeps every wait inside the kernel to 512 of K.
+  const bool parts = g.K > (out_bf16 ? kLongBf16 : kLongBlocks * kBK);
+  const int bn = linear_tile(g.M, g.N, g.K, out_bf16 && !parts, linear_plain(g.act), parts, g.resid != nullptr);
   CUtensorMap ta, tb, to;
   if (!make_kmajor_map(&ta, g.A, g.M, g.K, lda, kBM)) return -2;
   if (!make_kmajor_map(&tb, g.W, g.N, g.K, ldw, bn == 256 ? 128 : bn)) return -2;
   std::memset(&to, 0, sizeof(to));
-  if (out_bf16 && e.aligned &&
+  if (out_bf16 && e.aligned && !parts &&
       !make_tma_2d_bf16_swizzled(&to, g.out, g.M, g.N, g.M == 1 ? g.N : g.ldo, 32, 32, 64))
     return -2;
   auto launch = [&](auto act) {
     constexpr int ACT = decltype(act)::value;
+    if (out_bf16 && parts)
+      return launch_linear<INL_EPI_LINEAR_BF16_LONG, kLinearAny>(bn, ta, tb, to, g.M, g.N, g.K, e, g.status, stream);
     return out_bf16 ? launch_linear<INL_EPI_LINEAR_BF16, ACT>(bn, ta, tb, to, g.M, g.N, g.K, e, g.status, stream)
            : parts  ? launch_linear<INL_EPI_LINEAR_F32_LONG, ACT>(bn, ta, tb, to, g.M, g.N, g.K, e, g.status, stream)
                     : launch_linear<INL_EPI_LINEAR_F32, ACT>(bn, ta, tb, to, g.M, g.N, g.K, e, g.status, stream);

@@ -26,6 +26,7 @@ enum InlEpilogue : int {
   INL_EPI_LINEAR_BF16 = 8, // out = bf16(act(r * acc + bias) + resid); bias and resid (bf16) may be null
   INL_EPI_LINEAR_F32 = 9,  // the same with an f32 output and residual
   INL_EPI_LINEAR_F32_LONG = 10,  // and the sum moved out of TMEM every 512 of K (see gemm_bf16_linear)
+  INL_EPI_LINEAR_BF16_LONG = 11, // the same of INL_EPI_LINEAR_BF16
 };
 
 // Columns per partial sum of squares written by the residual epilogue.

@@ -523,3 +523,26 @@ def test_long_sums_of_one_sign(gpu, M, N, dt, odd, K):
     rel = ((out.double() - want).norm() / want.norm()).item()
     limit = (33 + (K / 512) ** 0.5) * U if dt == BF16 else (17 + 20 + (K / 128) ** 0.5) * U
     assert rel <= limit, (rel / U, limit / U)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N", [(1024, 1024), (2048, 640), (1030, 1001)])
+def test_long_sums_of_one_sign_in_bf16(gpu, M, N):
+    """A bf16 result is the exact sum's rounding but where that lies within the sum's own error e (as above) of a border
+    between two: of values spread over their binade, 2 e to a step of 2^-8 of the value at least."""
+    import torch
+
+    n = _n()
+    K = 1 << 17
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = ((torch.rand(M, K, generator=g, device="cuda") + 0.5) * (1 + torch.rand(M, 1, generator=g, device="cuda"))).bfloat16()
+    w = (torch.rand(N, K, generator=g, device="cuda") + 0.5).bfloat16()
+    for resid in (False, True):
+        r = torch.zeros(M, N, device="cuda", dtype=torch.bfloat16) if resid else None
+        out, st = torch.empty(M, N, device="cuda", dtype=torch.bfloat16), torch.zeros(1, dtype=torch.int32, device="cuda")
+        n.check(_call(n, torch, x, w, BF16, BF16, "relu", None, r, out, status=st), "linear")
+        want = sum(x[:, k:k + 8192].double() @ w[:, k:k + 8192].double().T for k in range(0, K, 8192))
+        assert st.item() == 0
+        off = (out != want.bfloat16()).double().mean().item()
+        assert off <= 2 * (33 + (K / 512) ** 0.5) * U / 2 ** -8, off
+        assert ((out.double() - want).abs() <= 2.0 ** -8 * want).all()
