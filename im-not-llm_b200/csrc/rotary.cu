@@ -20,6 +20,7 @@
 #include "common.cuh"
 #include "hook_checks.h"
 #include "kernels.h"
+#include "turns.h"
 
 namespace inl {
 
@@ -54,37 +55,6 @@ template <typename T>
 __device__ __forceinline__ void store_f(T* p, float v) {
   if constexpr (sizeof(T) == 2) *p = __float2bfloat16_rn(v);
   else *p = v;
-}
-
-// inv_freq (radians per position) as a fraction of a turn per position in
-// 2^-64 turns: pos times it, modulo 2^64, is where the angle ends in its turn,
-// exactly, for any 32-bit position, by one integer product.
-__device__ __forceinline__ uint64_t turn_step(double inv_freq) {
-  const double turns = inv_freq * 0.15915494309189533577;  // 1 / (2 pi)
-  return static_cast<uint64_t>((turns - floor(turns)) * 18446744073709551616.0);
-}
-
-// cos and sin of the angle pos * step: the quarter turn nearest to it by
-// integer arithmetic, and the rest, at most an eighth of a turn, by the Taylor
-// polynomials (the first terms left out are below 2e-9).
-__device__ __forceinline__ void turn_of(int pos, uint64_t step, float& c, float& s) {
-  const int t = static_cast<int>((static_cast<uint64_t>(static_cast<long long>(pos)) * step) >> 32);
-  const int k = (t + (1 << 29)) >> 30;  // wraps to the same quarter at half a turn
-  const float x = static_cast<float>(static_cast<int>(static_cast<unsigned>(t) - (static_cast<unsigned>(k) << 30))) *
-                  1.4629180792671596e-9f;  // 2 pi / 2^32
-  const float x2 = x * x;
-  float cr = fmaf(x2, -1.f / 3628800.f, 1.f / 40320.f);
-  cr = fmaf(x2, cr, -1.f / 720.f);
-  cr = fmaf(x2, cr, 1.f / 24.f);
-  cr = fmaf(x2, cr, -0.5f);
-  cr = fmaf(x2, cr, 1.f);
-  float sr = fmaf(x2, 1.f / 362880.f, -1.f / 5040.f);
-  sr = fmaf(x2, sr, 1.f / 120.f);
-  sr = fmaf(x2, sr, -1.f / 6.f);
-  sr = fmaf(x2 * x, sr, x);
-  const float p = (k & 1) ? sr : cr, q = (k & 1) ? cr : sr;
-  c = ((k + 1) & 2) ? -p : p;
-  s = (k & 2) ? -q : q;
 }
 
 // Any head width, stride and alignment: a warp per (token, head), a lane per

@@ -92,3 +92,14 @@ def test_host_layer_under_thread_sanitizer(tmp_path):
     _run([GXX, *flags, str(HOST / "engine.cpp"), str(ROOT / "tests" / "cpp" / "test_engine.cpp"), "-o", str(exe)])
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "all passed" in r.stdout and "WARNING: ThreadSanitizer" not in r.stderr, r.stderr
+
+
+def test_rotary_angles_without_undefined_behaviour(tmp_path):
+    """csrc/turns.h, the rotary kernels' angles, on the host under UBSan."""
+    exe = tmp_path / "test_turns"
+    flags = [*FLAGS, "-ffp-contract=off", f"-I{ROOT / 'im-not-llm_b200' / 'csrc'}"]
+    ub = [*flags, "-g", "-fsanitize=undefined,float-cast-overflow", "-fno-sanitize-recover=all"]
+    probe = subprocess.run([GXX, *ub, "-x", "c++", "-", "-o", str(tmp_path / "probe")], input="int main(){}",
+                           capture_output=True, text=True, timeout=120)
+    _run([GXX, *(ub if probe.returncode == 0 else flags), str(ROOT / "tests" / "cpp" / "test_turns.cpp"), "-o", str(exe)])
+    assert "all passed" in _run([str(exe)])
