@@ -406,7 +406,8 @@ int bad(const char* what, const char* why) {
 // Checks that need no device. Row widths as 64-bit products.
 int check_rotary(const char* what, int dtype, int T, int d, int rot, const RotaryArgs& a) {
   if (dtype != INL_DTYPE_F32 && dtype != INL_DTYPE_BF16) return bad(what, "dtype is f32 or bf16");
-  if (T < 0 || T > 1 << 30 || d <= 0) return bad(what, "T from 0 to 2^30, d > 0");
+  // a lane's feature index steps past d by up to 32
+  if (T < 0 || T > 1 << 30 || d <= 0 || d > 1 << 30) return bad(what, "T from 0 to 2^30, d from 1 to 2^30");
   if (rot < 0 || rot > d || (rot & 1)) return bad(what, "rotary_dim is even and at most d");
   if (!std::isfinite(a.scale)) return bad(what, "scale is finite");
   for (const HeadSet& h : a.set) {

@@ -256,7 +256,7 @@ INL_API int inl_cuda_rope_frequencies(const inl_rope_config* config, double* inv
  * pair i being features (i, i + rotary_dim / 2), or (2i, 2i + 1) when
  * `interleaved`; the other features are copied. `inverse` rotates by -t (the
  * transpose: undoes a rotation of scale 1, and carries a gradient back).
- * T up to 2^30, heads up to 65536. pos: device int32 [T], any sign; inv_freq: device f64
+ * T and d up to 2^30, heads up to 65536. pos: device int32 [T], any sign; inv_freq: device f64
  * [rotary_dim / 2], finite; the angle is formed modulo one turn in 64 bits, so far
  * positions lose nothing and there is no table. out may be x itself (same pointer and
  * stride) and overlaps it in no other way. Element-aligned pointers, strides

@@ -177,6 +177,16 @@ def test_qk_refusals_need_no_gpu():
     assert call(hq=0, hkv=0, q=None, k=None, qo=None, ko=None) == 0
 
 
+@pytest.mark.parametrize("d", [(1 << 30) + 1, (1 << 31) - 1])
+def test_heads_past_32_bit_feature_indices_are_refused(d):
+    n = _n()
+    assert n.lib().inl_cuda_rope(16, d, BF16, 1, 1, d, 64, 0, 16, 16, 1.0, 0, 64, d, None) == INVALID
+    assert n.last_error() == "rope: T from 0 to 2^30, d from 1 to 2^30"
+    assert n.lib().inl_cuda_qk_norm_rotary(16, d, d, 16, d, BF16, 1, 1, 1, d, 0, None, None, None, None, 1e-6, 64, 0, 16, 16, 1.0,
+                                           64, d, 64, d, None) == INVALID
+    assert n.last_error() == "qk_norm_rotary: T from 0 to 2^30, d from 1 to 2^30"
+
+
 # ---------------------------------------------------------------- GPU
 def _rot64(torch, y, pos, freq, scale, rot, inter, inverse=False):
     """(rotated, sum of the pair's magnitudes) of y [T, heads, d] in 64 bits."""
