@@ -546,3 +546,28 @@ def test_long_sums_of_one_sign_in_bf16(gpu, M, N):
         off = (out != want.bfloat16()).double().mean().item()
         assert off <= 2 * (33 + (K / 512) ** 0.5) * U / 2 ** -8, off
         assert ((out.double() - want).abs() <= 2.0 ** -8 * want).all()
+
+
+# The residual stream updated in place, through every path that reads the residual ahead of its products or stores: tiles
+# of 64 to 256 columns, K in one part and in several, clusters, few rows, rows of odd strides, ragged last tiles.
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["none", "relu", "gelu_tanh"])
+@pytest.mark.parametrize("dt,odt,odd", [(BF16, BF16, 0), (BF16, F32, 0), (BF16, BF16, 1), (BF16, F32, 1), (F32, F32, 0),
+                                        (F32, BF16, 0), (F32, F32, 1)])
+@pytest.mark.parametrize("M,N,K", [(1, 520, 136), (16, 1176, 136), (30, 5000, 136), (64, 1152, 328), (100, 1000, 1032),
+                                   (250, 704, 400), (500, 2304, 392), (500, 2304, 776), (2001, 1000, 200),
+                                   (2001, 1000, 1000), (4205, 760, 264), (4205, 760, 520), (1283, 584, 1160),
+                                   (1003, 4088, 1096), (515, 515, 72), (70, 264, 33000)])
+def test_the_residual_updated_in_place(gpu, M, N, K, dt, odt, odd, act):
+    import torch
+
+    n = _n()
+    x, _ = _rows(torch, M, K, odd, dt, 3)
+    w, _ = _rows(torch, N, K, odd, dt, 4, K ** -0.5)
+    b = torch.randn(N, generator=torch.Generator().manual_seed(6)).cuda()
+    r, frame = _rows(torch, M, N, 16 + odd, odt, 5)
+    r0, st = r.clone(), torch.zeros(1, dtype=torch.int32, device="cuda")
+    n.check(_call(n, torch, x, w, dt, odt, act, b, r, r, status=st), "linear")
+    torch.cuda.synchronize()
+    assert st.item() == 0 and torch.isnan(frame.view(M, -1)[:, N:]).all()
+    _check(torch, r, x, w, b, act, r0, odt)
