@@ -74,17 +74,17 @@ __device__ __forceinline__ float act_exact(float v, int act) {
   }
 }
 
-// gelu(x) = x Phi(x) for a result that is rounded to bf16: erfc by the rational
-// form 7.1.26 of Abramowitz and Stegun (absolute error 1.5e-7), on its own side
-// of zero, so that the tail of a negative x keeps its size.
+// gelu(x) = x Phi(x) for a result that is rounded to bf16: normal_tail with a fit
+// of 2^-20.6 of the value, on the tail too.
 __device__ __forceinline__ float gelu_erf_fast(float x) {
-  const float z = fabsf(x) * 0.70710678f;
-  const float t = rcp_approx(fmaf(0.3275911f, z, 1.0f));
-  float p = fmaf(1.061405429f, t, -1.453152027f);
-  p = fmaf(p, t, 1.421413741f);
-  p = fmaf(p, t, -0.284496736f);
-  p = fmaf(p, t, 0.254829592f);
-  const float tail = 0.5f * p * t * ex2_approx(z * z * -1.44269504f);  // Phi(-|x|)
+  const float y = fabsf(x), t = rcp_approx(fmaf(0.265f, y, 1.0f));
+  float p = fmaf(-0.0677870288f, t, 0.195273072f);
+  p = fmaf(p, t, -0.0663628653f);
+  p = fmaf(p, t, 0.142493308f);
+  p = fmaf(p, t, 0.0829465985f);
+  p = fmaf(p, t, 0.107836775f);
+  p = fmaf(p, t, 0.105599836f);
+  const float tail = p * t * ex2_approx(y * y * -0.72134752f);
   return x * (x < 0.f ? tail : 1.0f - tail);
 }
 // 0.5 (1 + tanh(u)) = 1 / (1 + exp(-2 u)).

@@ -571,3 +571,27 @@ def test_the_residual_updated_in_place(gpu, M, N, K, dt, odt, odd, act):
     torch.cuda.synchronize()
     assert st.item() == 0 and torch.isnan(frame.view(M, -1)[:, N:]).all()
     _check(torch, r, x, w, b, act, r0, odt)
+
+
+# A bf16 result's gelu (erf): 2^-19 of the value (the fit, the exponential's argument at most (x^2 + 1) 2^-23 = 2^-17 at -8)
+# before one rounding, where the sum is exact (x is zero, the bias is it). Values from -8 up, so the tail counts.
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,M,K", [(BF16, 3, 64), (BF16, 130, 1024), (BF16, 700, 64), (F32, 3, 64), (F32, 1500, 64),
+                                    (BF16, 150, 61)])
+def test_bf16_gelu_keeps_its_digits_on_the_tail(gpu, dt, M, K):
+    import math
+
+    import torch
+
+    n = _n()
+    N = 1504
+    x = torch.zeros(M, K, device="cuda", dtype=_dt(torch, dt))
+    w = torch.ones(N, K, device="cuda", dtype=_dt(torch, dt))
+    v = torch.linspace(-8, 3, N, device="cuda")
+    out = torch.empty(M, N, device="cuda", dtype=torch.bfloat16)
+    n.check(_call(n, torch, x, w, dt, BF16, "gelu_erf", v, None, out), "linear")
+    torch.cuda.synchronize()
+    z = v.double()
+    want = 0.5 * z * torch.special.erfc(-z / math.sqrt(2))
+    before = (2.0 ** -19 + (z * z + 1) * 2.0 ** -23) * want.abs()
+    assert ((out.double() - want).abs() <= before * (1 + 2.0 ** -8) + 2.0 ** -8 * want.abs() + 1e-37).all()
