@@ -52,6 +52,18 @@ __device__ __forceinline__ float2 unpack_bf16x2(uint32_t v) {
   return __bfloat1622float2(b);
 }
 
+// A bf16 or f32 value as f32, and back.
+template <typename T>
+__device__ __forceinline__ float load_f(const T* p) {
+  if constexpr (sizeof(T) == 2) return __bfloat162float(*p);
+  else return *p;
+}
+template <typename T>
+__device__ __forceinline__ void store_f(T* p, float v) {
+  if constexpr (sizeof(T) == 2) *p = __float2bfloat16_rn(v);
+  else *p = v;
+}
+
 // ---------------------------------------------------------------- mbarrier
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));

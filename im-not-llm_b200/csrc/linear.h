@@ -20,17 +20,6 @@ struct LinearArgs {
   int M, N, K, act;
 };
 
-template <typename T>
-__device__ __forceinline__ float load_f(const T* p) {
-  if constexpr (sizeof(T) == 2) return __bfloat162float(*p);
-  else return *p;
-}
-template <typename T>
-__device__ __forceinline__ void store_f(T* p, float v) {
-  if constexpr (sizeof(T) == 2) *p = __float2bfloat16_rn(v);
-  else *p = v;
-}
-
 // Phi(-y), y >= 0, to f32 accuracy relative to itself: exp(-y^2 / 2) times a
 // polynomial in t = 1 / (1 + 0.4 y), the form of 7.1.26 of Abramowitz and Stegun
 // with a minimax fit of its own (2^-26 of the value up to y = 14.5). The argument

@@ -46,17 +46,6 @@ struct RotaryArgs {
   const double* inv_freq;
 };
 
-template <typename T>
-__device__ __forceinline__ float load_f(const T* p) {
-  if constexpr (sizeof(T) == 2) return __bfloat162float(*p);
-  else return *p;
-}
-template <typename T>
-__device__ __forceinline__ void store_f(T* p, float v) {
-  if constexpr (sizeof(T) == 2) *p = __float2bfloat16_rn(v);
-  else *p = v;
-}
-
 // Any head width, stride and alignment: a warp per (token, head), a lane per
 // pair (and per feature that is copied), so that in-place rows are read and
 // written by one lane alone. Two passes over the head when it is normed.
