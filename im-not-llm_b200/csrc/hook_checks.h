@@ -29,9 +29,10 @@ inline int check_aligned(const char* what, std::initializer_list<HookPtr> ptrs) 
   return INL_OK;
 }
 
-// Memory the current device can read: its own, managed, or pinned host
-// memory. A pageable host pointer or another device's memory is refused here,
-// since a kernel that touches it would fault and take the context with it.
+// Memory of the current device, managed memory or pinned host memory. The rest
+// is refused, since a kernel that touches it may fault and take the context with
+// it: pageable host memory, and another device's, of which a pointer does not
+// tell whether this device was given access to it.
 inline int check_reachable(const char* what, std::initializer_list<HookPtr> ptrs) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);

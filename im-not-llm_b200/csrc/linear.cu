@@ -33,8 +33,9 @@ __device__ __forceinline__ void load_values(const T* row, int k, int K, float (&
 // A read of w, like linear_skinny_kernel, on FFMA: a CTA owns R rows of w and MT
 // rows of x, its 8 warps take turns of K, a lane V values of each row. f32 sums:
 // over a lane's share of K, then the lanes and the warps in order. One f32 row
-// x 1024 x 1024: 2.6 us; x 4096 x 1024: 6.0 us = 2.8 TB/s; 8 rows of the
-// latter 13.5 us, bound by the loads of x, which every CTA makes again.
+// x 1024 x 1024: 2.6 us; x 4096 x 1024: 6.0 us = 2.8 TB/s (w in L2; 7.4 from
+// memory); 4 rows of the latter 10 us, with 39 words a thread spilled at three
+// CTAs an SM; 8 rows 13.5 us, bound by the loads of x, which every CTA makes again.
 template <typename TX, typename TO, int MT, int R, int V>
 __global__ void __launch_bounds__(256, MT < 8 ? 3 : 2) linear_rows_kernel(LinearArgs g) {
   __shared__ float red[8][MT * R];

@@ -298,7 +298,8 @@ __device__ __forceinline__ void cluster_finish(const LinearArgs& g, uint8_t* par
 // PLAIN (f32 results without an activation's special functions): the bias and 4
 // PLAIN rows of the residual are asked for before the turn. bf16 to f32 with a
 // residual: 16384 x 1024 x 512 47.6 -> 34.9 us (PLAIN 8), 65536 x 768 x 768, K in
-// parts, 144 -> 124 (4; 8 spills: 130); beside gelu it spilled, 37 -> 45.
+// parts, 144 -> 124 (4: the 192- and 256-wide kernels, whose sums are 96 and 128
+// registers, spill 29 and 222 words; 8: 130); beside gelu 37 -> 45.
 template <typename TO, bool REDO, int PLAIN = 0>
 __device__ __forceinline__ void warp_finish32(const LinearArgs& g, uint8_t* buf, const float* v, int m, int n, int lane,
                                               bool wide) {

@@ -24,7 +24,7 @@
 // where the products alone, the splitting left out, take 1.19 ms at the clock
 // that the power limit leaves. With both operands split in shared memory, 72 us
 // on the first: the tile's 224 KB of shared memory traffic a K block bound it; one
-// tile to a CTA 62 us. Rows of odd strides: 92 us.
+// tile to a CTA 62 us. Rows of odd strides: 97 us.
 #include <algorithm>
 #include <type_traits>
 

@@ -180,18 +180,29 @@ INL_API int inl_cuda_gated_delta_rule(const float* mixed, int64_t ld_mixed, cons
                                       void* stream);
 
 /* Linear layer: out[M, N] = act(x[M, K] . w[N, K]^T + bias[N]) + resid[M, N],
- * sums, bias, activation and residual in f32 and one rounding at the end.
+ * sums, bias, activation and residual in f32 and one rounding at the end. The
+ * tensor cores truncate as they add, so long sums come in parts of 128 to 512 of K
+ * that are added to nearest: f32 results of bf16 operands are off by 1e-7 to
+ * 3e-7 of sum |x w|, of f32 operands by 4e-7 to 6e-7 (K from 1024 to 2^20,
+ * measured); parts of sums for bf16 results start at K = 32768 (3e-5 there, a 60th
+ * of half a step). Activations of f32 results are off by some 2^-24 of
+ * their value (2^-16 on gelu's tail at -8, an exponential's argument rounded),
+ * those of bf16 results by 2^-20 of their argument.
  * `dtype` (INL_DTYPE_*) is that of x and w; `out_dtype` that of out and resid;
  * bias is f32; bias and resid may be NULL. act is any INL_ACT_*_. Any
  * M, N, K from 0 to 2^30 (K = 0: the product is zero; M * N up to 2^40), any
  * row strides >= the row length, element-aligned pointers; rows of x and w on
- * 16-byte boundaries are the fast case. f32 operands give f32 accuracy (they
+ * 16-byte boundaries are the fast case. f32 operands
  * are split for the tensor cores, each to 2^-21 of itself or 2^-137, whichever is
- * more; a sum that comes out NaN is computed again in plain f32, so infinities
- * keep to their rows as they would). out may be
+ * more (a sum of one or two products is that far off, a plain f32 one 2^-24; from
+ * 32 products on it is the closer one); a sum that comes out NaN is computed
+ * again in plain f32, so infinities keep to their rows as they would, at 0.14 us an
+ * element of K for every sum that holds one. out may be
  * resid itself (same pointer and stride); it overlaps nothing else. Nothing
  * outside the [M, N] elements of out is written. `status` as for
- * inl_cuda_gemm_bf16. Memory must be reachable from the current device.
+ * inl_cuda_gemm_bf16. Pointers are to memory of the current device, managed
+ * memory or pinned host memory; others (another device's, peer access or not, and
+ * pageable host memory, also where the device could read it) are refused.
  * Asynchronous on `stream`, no allocation, may be captured. Results do not
  * change from run to run; they may differ by rounding between M, since the
  * kernel is chosen by the sizes. Replaces candle_nn::Linear::forward with a
@@ -259,8 +270,8 @@ INL_API int inl_cuda_rope_frequencies(const inl_rope_config* config, double* inv
  * T and d up to 2^30, heads up to 65536. pos: device int32 [T], any sign; inv_freq: device f64
  * [rotary_dim / 2], finite; the angle is formed modulo one turn in 64 bits, so far
  * positions lose nothing and there is no table. out may be x itself (same pointer and
- * stride) and overlaps it in no other way. Element-aligned pointers, strides
- * >= heads * d. Asynchronous on `stream`, no allocation, may be captured.
+ * stride) and overlaps it in no other way. Element-aligned pointers (memory as for
+ * inl_cuda_linear), strides >= heads * d. Asynchronous on `stream`, no allocation, may be captured.
  * Replaces candle_nn::rotary_emb::rope and rope_i. */
 INL_API int inl_cuda_rope(const void* x, int64_t ldx, int dtype, int T, int heads, int d, int rotary_dim,
                           int interleaved, const int32_t* pos, const double* inv_freq, float scale, int inverse,
@@ -276,7 +287,8 @@ INL_API int inl_cuda_rope(const void* x, int64_t ldx, int dtype, int T, int head
  * q | gate rows of gated attention), k head h at k + t * ldk + h * d; outputs
  * have heads at h * d. hq or hkv may be 0 (its pointers are not read). q_out
  * may be q itself when the strides are equal and q_head_stride = d, k_out may
- * be k itself; nothing overlaps in any other way. Replaces q_norm / k_norm +
+ * be k itself; nothing overlaps in any other way. Sizes and memory as for
+ * inl_cuda_rope. Replaces q_norm / k_norm +
  * rotary_emb::rope (crates/inl-text/src/qwen3/mod.rs:236-249) and the partial
  * form of crates/inl-late/src/qwen3_5.rs. */
 INL_API int inl_cuda_qk_norm_rotary(const void* q, int64_t ldq, int64_t q_head_stride, const void* k, int64_t ldk,

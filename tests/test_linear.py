@@ -595,3 +595,11 @@ def test_bf16_gelu_keeps_its_digits_on_the_tail(gpu, dt, M, K):
     want = 0.5 * z * torch.special.erfc(-z / math.sqrt(2))
     before = (2.0 ** -19 + (z * z + 1) * 2.0 ** -23) * want.abs()
     assert ((out.double() - want).abs() <= before * (1 + 2.0 ** -8) + 2.0 ** -8 * want.abs() + 1e-37).all()
+
+
+# bf16 results of long K, whose sums come in parts: tiles of 64, 128, 192 and the pair's 256 columns, rows of any alignment
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,resid,pad", [(1024, 1024, True, 0), (1500, 1500, True, 0), (2040, 1728, False, 8),
+                                           (2048, 2040, True, 0), (2000, 1999, True, 3)])
+def test_bf16_results_of_long_k(gpu, M, N, resid, pad):
+    _one(M, N, 32776, BF16, BF16, "gelu_erf", True, resid, pad=(0, 0, pad, pad), seed=51)
