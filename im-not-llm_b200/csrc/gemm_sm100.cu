@@ -37,7 +37,9 @@ constexpr int kEpiWarps = 8;  // two warps per TMEM lane quadrant, each owning h
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kLongBlocks = 8;  // K blocks between promotions of the sum (epi_long)
 constexpr int kLongBf16 = 32768;  // K past which a bf16 result takes them
-__host__ __device__ constexpr bool epi_long(int epi) { return epi == INL_EPI_LINEAR_F32_LONG || epi == INL_EPI_LINEAR_BF16_LONG; }
+__host__ __device__ constexpr bool epi_long(int epi) {
+  return epi == INL_EPI_LINEAR_F32_LONG || epi == INL_EPI_LINEAR_BF16_LONG;
+}
 
 template <int BN>
 struct GemmCfg {
@@ -507,7 +509,8 @@ __device__ __forceinline__ void epilogue_tile(uint32_t t_row, int row, int n0, i
   }
 }
 
-// The epilogue of one tile whose sum comes in parts of K (epi_long), for one warp: this thread's row, half of the columns, summed in registers.
+// The epilogue of one tile whose sum comes in parts of K (epi_long), for one
+// warp: this thread's row, half of the columns, summed in registers.
 // `taken(acc)` gives accumulator acc back. False: a wait ran out.
 template <int BN, int EPI, bool PLAIN, typename Taken>
 __device__ __forceinline__ bool epilogue_long(uint32_t tmem, uint64_t* tfull, int& acc, uint32_t& acc_phase, int parts,

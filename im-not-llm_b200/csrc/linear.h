@@ -67,7 +67,7 @@ __device__ __forceinline__ float act_exact(float v, int act) {
 // of 2^-20.6 of the value, on the tail too.
 __device__ __forceinline__ float gelu_erf_fast(float x) {
   const float y = fabsf(x), t = rcp_approx(fmaf(0.265f, y, 1.0f));
-  float p = fmaf(-0.0677870288f, t, 0.195273072f);
+  float p = fmaf(-0.0677870288f, t, 0.19527307f);
   p = fmaf(p, t, -0.0663628653f);
   p = fmaf(p, t, 0.142493308f);
   p = fmaf(p, t, 0.0829465985f);

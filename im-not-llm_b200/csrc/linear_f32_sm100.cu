@@ -160,7 +160,9 @@ __global__ void __launch_bounds__(threads_of(TMA), 1)
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
     return TMA ? wait_alive(bar, parity, status, code) : mbar_wait(bar, parity, status, code);
   };
-  auto wait_warp = [&](uint64_t* bar, uint32_t parity, int code) { return __all_sync(0xffffffffu, wait(bar, parity, code)); };
+  auto wait_warp = [&](uint64_t* bar, uint32_t parity, int code) {
+    return __all_sync(0xffffffffu, wait(bar, parity, code));
+  };
 
   if (warp == 0) {
     if (TMA && lane == 0) {

@@ -27,7 +27,8 @@ INL_HOST_DEVICE uint64_t turn_step(double inv_freq) {
 // polynomials (the first terms left out are below 2e-9).
 INL_HOST_DEVICE void turn_of(int pos, uint64_t step, float& c, float& s) {
   const int t = static_cast<int>((static_cast<uint64_t>(static_cast<long long>(pos)) * step) >> 32);
-  const int k = static_cast<int>(static_cast<unsigned>(t) + (1u << 29)) >> 30;  // wraps to the same quarter at half a turn
+  // wraps to the same quarter at half a turn
+  const int k = static_cast<int>(static_cast<unsigned>(t) + (1u << 29)) >> 30;
   const float x = static_cast<float>(static_cast<int>(static_cast<unsigned>(t) - (static_cast<unsigned>(k) << 30))) *
                   1.4629180792671596e-9f;  // 2 pi / 2^32
   const float x2 = x * x;
